@@ -15,6 +15,7 @@
 #include "dml_comm.h"
 #include "dml_engine.h"
 #include "dml_kernels.h"
+#include "dml_newton_schulz.h"
 
 namespace py = pybind11;
 namespace dml {
@@ -276,6 +277,40 @@ PYBIND11_MODULE(_C, m) {
         sgd_momentum(ptr<float>(p), ptr<const float>(g), ptr<float>(mom), ptr<bf16_raw>(shadow), n,
                      lr, mu, wd, gscale, first, st(s));
     });
+    // matrices: (rows, cols, batch, offset, ld, stride, out_offset, out_ld, out_stride, lr) each
+    typedef std::tuple<int, int, int, long long, long long, long long, long long, long long, long long,
+                       float> NsTuple;
+    py::class_<NewtonSchulzPlan>(m, "NewtonSchulzPlan")
+        .def(py::init([](const std::vector<NsTuple>& matrices,
+                         const std::vector<std::pair<long long, long long>>& segments,
+                         const std::vector<float>& coefficients, double eps, bool wide_products) {
+            std::vector<NsShape> shapes;
+            for (const NsTuple& t : matrices) {
+                NsShape s;
+                std::tie(s.rows, s.cols, s.batch, s.offset, s.ld, s.stride, s.out_offset, s.out_ld,
+                         s.out_stride, s.lr) = t;
+                shapes.push_back(s);
+            }
+            std::vector<NsSegment> segs;
+            for (const auto& g : segments) segs.push_back(NsSegment{g.first, g.second});
+            return new NewtonSchulzPlan(shapes, segs, coefficients, eps, wide_products);
+        }))
+        .def_property_readonly("workspace_bytes", &NewtonSchulzPlan::workspace_bytes)
+        .def("orthogonalize", [](const NewtonSchulzPlan& n, uintptr_t x, uintptr_t out, int type,
+                                 uintptr_t ws, size_t ws_bytes, uintptr_t s) {
+            if (type < NS_F32 || type > NS_F16) throw std::invalid_argument("newton_schulz: element type");
+            n.orthogonalize(ptr<const void>(x), ptr<void>(out), (NsType)type, ptr<void>(ws), ws_bytes, st(s));
+        })
+        .def("muon", [](const NewtonSchulzPlan& n, uintptr_t p, uintptr_t g, uintptr_t mom, float lr,
+                        float momentum, float weight_decay, bool nesterov, float sgd_lr,
+                        float sgd_momentum, float sgd_weight_decay, float grad_scale, uintptr_t ws,
+                        size_t ws_bytes, uintptr_t s) {
+            MuonArgs a;
+            a.lr = lr; a.momentum = momentum; a.weight_decay = weight_decay; a.nesterov = nesterov;
+            a.sgd_lr = sgd_lr; a.sgd_momentum = sgd_momentum; a.sgd_weight_decay = sgd_weight_decay;
+            a.grad_scale = grad_scale;
+            n.muon(ptr<float>(p), ptr<const float>(g), ptr<float>(mom), a, ptr<void>(ws), ws_bytes, st(s));
+        });
     m.def("cast_f32_to_bf16", [](uintptr_t x, uintptr_t out, size_t n, uintptr_t s) {
         cast_f32_to_bf16(ptr<const float>(x), ptr<bf16_raw>(out), n, st(s));
     });

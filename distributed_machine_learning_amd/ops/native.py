@@ -10,6 +10,7 @@ to build it, so a GPU run can never silently use stock torch ops.
 """
 from __future__ import annotations
 
+import functools
 import os
 from typing import Optional, Tuple
 
@@ -497,6 +498,160 @@ def sgd_momentum_(p: torch.Tensor, g: torch.Tensor, m: torch.Tensor, lr: float, 
             raise ValueError("sgd_momentum_: shadow too small")
     lib().sgd_momentum(p.data_ptr(), g.data_ptr(), m.data_ptr(), _ptr(shadow), p.numel(), lr,
                        momentum, weight_decay, grad_scale, first_step, _stream())
+
+
+# ------------------------------------------------------------- orthogonalised updates
+# The quintic whose five-fold iteration sends singular values of (0, 1] to about 1.
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+_NS_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+NS_PRECISIONS = ("fp32", "fp16")
+
+
+def ns_coefficients(steps: int, coefficients) -> Tuple[float, ...]:
+    """Flat ``(a, b, c)`` per step from one triple or a sequence of ``steps`` triples."""
+    steps = int(steps)
+    if not 1 <= steps <= 64:
+        raise ValueError(f"newton_schulz: steps must be 1 .. 64, got {steps}")
+    c = list(coefficients)
+    if len(c) == 3 and all(isinstance(v, (int, float)) for v in c):
+        c = [c] * steps
+    if len(c) != steps or any(len(t) != 3 for t in c):
+        raise ValueError(f"newton_schulz: coefficients are one (a, b, c) or one for each of the {steps} steps")
+    return tuple(float(v) for t in c for v in t)
+
+
+def _ns_wide(precision: Optional[str], dtype: torch.dtype, smallest: int) -> bool:
+    """Whether the products keep 22 bits of their factors ("fp32") or 11 ("fp16")."""
+    if precision is None:
+        # 11 bits per factor serve a result that is rounded to 8.  Below ~128 rows the rounding no
+        # longer averages out (1e-2 of a [10, 512] result) and the products cost next to nothing.
+        return dtype != torch.bfloat16 or smallest <= 128
+    if precision not in NS_PRECISIONS:
+        raise ValueError(f"newton_schulz: precision must be one of {NS_PRECISIONS}, got {precision!r}")
+    return precision == "fp32"
+
+
+@functools.lru_cache(maxsize=256)
+def _ns_plan(matrices, segments, coefficients, eps, wide):
+    """Plans hold shapes and launch parameters only (no memory), so equal calls share one."""
+    return lib().NewtonSchulzPlan(list(matrices), list(segments), list(coefficients), eps, wide)
+
+
+def _ns_layout(x: torch.Tensor):
+    """``(batch, rows, cols, ld, stride, transposed)`` of ``x`` as batches of matrices with
+    contiguous rows in memory, or None if its strides do not allow that."""
+    m, n = x.shape[-2:]
+    sm, sn = x.stride(-2), x.stride(-1)
+    if (sn == 1 or n == 1) and (sm >= n or m == 1):
+        rows, cols, ld, transposed = m, n, (sm if m > 1 else n), False
+    elif (sm == 1 or m == 1) and (sn >= m or n == 1):
+        rows, cols, ld, transposed = n, m, (sn if n > 1 else m), True
+    else:
+        return None
+    batch, stride = 1, 0
+    for size, step in zip(reversed(x.shape[:-2]), reversed(x.stride()[:-2])):
+        if size == 1:
+            continue
+        if batch == 1:
+            stride = step
+        elif step != stride * batch:
+            return None
+        batch *= size
+    if batch > 1 and stride < 0:
+        return None
+    return batch, rows, cols, ld, stride, transposed
+
+
+def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
+                  precision: Optional[str] = None) -> torch.Tensor:
+    """``Y_0 = x / (||x||_F + eps)``, then ``steps`` times ``Y <- a Y + (b A + c A A) Y`` with
+    ``A = Y Y^T`` on the smaller side; ``x`` is ``[..., m, n]`` in fp32, bf16 or fp16 and the
+    result has its shape, type and row / column order.
+
+    Matrices with contiguous rows or columns and evenly spaced batches are read where they lie,
+    any other layout is copied first.  ``precision`` is that of the factors of the products:
+    ``"fp32"`` keeps 22 bits, ``"fp16"`` 11; sums, Y and the diagonals always keep at least 22.
+    The default is fp16 for bf16 matrices of more than 128 rows and columns, else fp32."""
+    if not x.is_cuda:
+        raise ValueError("newton_schulz: expected a GPU tensor")
+    if x.dtype not in _NS_TYPES:
+        raise TypeError(f"newton_schulz: expected fp32, bf16 or fp16, got {x.dtype}")
+    if x.dim() < 2:
+        raise ValueError(f"newton_schulz: expected [..., m, n], got {tuple(x.shape)}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("newton_schulz: has no gradient; pass x.detach() or call under torch.no_grad()")
+    coef = ns_coefficients(steps, coefficients)
+    wide = _ns_wide(precision, x.dtype, min(x.shape[-2:]))
+    if x.numel() == 0:
+        return torch.empty_like(x)
+    layout = _ns_layout(x)
+    if layout is None:
+        x = x.contiguous()
+        layout = _ns_layout(x)
+    batch, rows, cols, ld, stride, transposed = layout
+    out = torch.empty(*x.shape[:-2], rows, cols, dtype=x.dtype, device=x.device)
+    plan = _ns_plan(((rows, cols, batch, 0, ld, stride, 0, cols, rows * cols, 0.0),), (), coef,
+                    float(eps), wide)
+    with torch.cuda.device(x.device):
+        ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=x.device)
+        plan.orthogonalize(x.data_ptr(), out.data_ptr(), _NS_TYPES[x.dtype], ws.data_ptr(), ws.numel(),
+                           _stream())
+    return out.transpose(-2, -1) if transposed else out
+
+
+class MuonPlan:
+    """Which parts of flat fp32 buffers one :func:`muon_step_` updates, and how.
+
+    ``matrices``: ``(offset, rows, cols, lr_factor)`` of row-major matrices, ``segments``:
+    ``(offset, count)`` of everything that takes SGD with momentum; they must not overlap."""
+
+    def __init__(self, matrices, segments, steps: int = 5, coefficients=NS_COEFFICIENTS,
+                 eps: float = 1e-7, precision: str = "fp32"):
+        self.matrices = tuple((int(o), int(r), int(c), float(f)) for o, r, c, f in matrices)
+        self.segments = tuple((int(o), int(n)) for o, n in segments if n)
+        spans = sorted([(o, o + r * c) for o, r, c, _ in self.matrices] +
+                       [(o, o + n) for o, n in self.segments])
+        if any(lo < 0 or hi <= lo for lo, hi in spans) or \
+                any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("muon: matrices and segments must be non-empty, in order and disjoint")
+        self.elems = spans[-1][1] if spans else 0
+        self.coefficients = ns_coefficients(steps, coefficients)
+        self.eps = float(eps)
+        self.precision = precision
+        wide = _ns_wide(precision, torch.float32, 0)
+        self._plan = lib().NewtonSchulzPlan(
+            [(r, c, 1, o, c, 0, 0, 0, 0, f) for o, r, c, f in self.matrices], list(self.segments),
+            list(self.coefficients), self.eps, wide)
+        self.workspace_bytes = int(self._plan.workspace_bytes)
+
+
+def muon_step_(plan: MuonPlan, p: torch.Tensor, g: torch.Tensor, m: torch.Tensor, lr: float,
+               momentum: float, weight_decay: float, nesterov: bool = True, sgd_lr: float = 0.1,
+               sgd_momentum: float = 0.9, sgd_weight_decay: float = 1e-4, grad_scale: float = 1.0,
+               workspace: Optional[torch.Tensor] = None) -> None:
+    """In-place Muon update over flat fp32 buffers.  With ``g`` scaled by ``grad_scale``:
+
+    matrices: ``m = momentum * m + g``, ``u = g + momentum * m`` (``m`` without ``nesterov``),
+    ``p = (1 - lr * weight_decay) * p - lr * lr_factor * newton_schulz(u)``;
+    segments: ``g += sgd_weight_decay * p``, ``m = sgd_momentum * m + g``, ``p -= sgd_lr * m``.
+
+    A ``workspace`` (uint8, ``plan.workspace_bytes``) may be reused by calls ordered on one stream."""
+    for t, n in ((p, "p"), (g, "g"), (m, "m")):
+        _req(t, torch.float32, n, 1)
+        if t.device != p.device:
+            raise ValueError(f"muon_step_: {n} is on {t.device}, p on {p.device}")
+        if t.numel() != p.numel() or t.numel() < plan.elems:
+            raise ValueError(f"muon_step_: {n} has {t.numel()} elements, p {p.numel()}, the plan needs {plan.elems}")
+    if workspace is None:
+        workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=p.device)
+    else:
+        _req(workspace, torch.uint8, "workspace", 1)
+        if workspace.numel() < plan.workspace_bytes or workspace.device != p.device:
+            raise ValueError(f"muon_step_: workspace of {plan.workspace_bytes} bytes on {p.device} needed")
+    with torch.cuda.device(p.device):
+        plan._plan.muon(p.data_ptr(), g.data_ptr(), m.data_ptr(), lr, momentum, weight_decay, nesterov,
+                        sgd_lr, sgd_momentum, sgd_weight_decay, grad_scale, workspace.data_ptr(),
+                        workspace.numel(), _stream())
 
 
 # --------------------------------------------------------------- data and helpers
