@@ -12,6 +12,7 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <memory>
 #include <vector>
 
 namespace dml {
@@ -61,10 +62,11 @@ class NewtonSchulzPlan {
         int m, n, mp, np;
         long long ws, ws_stride;     // workspace of the first matrix and between matrices, bytes
     };
-    struct Launch;
+    struct Group;                    // the launches of as many matrices as a launch takes
     void check_workspace(const void* ws, size_t ws_bytes) const;
-    template <typename Prepare, typename Finish>
-    void chain(void* ws, hipStream_t stream, const Prepare& prepare, const Finish& finish) const;
+    template <typename Prepare>
+    void chain(char* ws, NsType type, const Prepare& prepare, void* out, float* p, float lr, float decay,
+               hipStream_t stream) const;
 
     std::vector<Matrix> mats_;
     std::vector<NsSegment> segs_;
@@ -72,7 +74,8 @@ class NewtonSchulzPlan {
     double eps_;
     bool wide_;
     int x_exp_, a_exp_, b_exp_;      // planes hold value * 2^exp
-    size_t ws_bytes_ = 0;
+    std::vector<std::shared_ptr<Group>> groups_;
+    size_t partials_ = 0, slab_ = 0, ws_bytes_ = 0;      // offsets in the workspace, its size
 };
 
 }  // namespace dml

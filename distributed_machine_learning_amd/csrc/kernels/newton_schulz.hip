@@ -15,7 +15,10 @@
 // Late in the iteration A is close to the identity, so the large part of both products is exact
 // and only the small off-diagonal part carries the narrow factors' rounding (measured against 64
 // bits on [512, 4608]: 1e-4 of the result's norm; with the diagonals left in, 3e-3).
+#include <algorithm>
 #include <cmath>
+#include <cstdio>
+#include <cstdlib>
 #include <stdexcept>
 #include <string>
 
@@ -29,10 +32,15 @@ typedef _Float16 f16_t;
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef const __attribute__((address_space(1))) void* global_ptr;
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 
-constexpr int kMaxProblems = 32;        // per launch: the table has to fit the kernel arguments
+constexpr int kMaxProblems = 24;        // per launch: the table has to fit the kernel arguments
 constexpr int kPad = 64;                // planes are zero-padded to multiples of this
-constexpr int kMaxPartials = 256;       // blocks (partial sums of squares) per matrix
+constexpr int kMaxPartials = 1024;      // blocks (partial sums of squares) per matrix
+constexpr int kCus = 256;
+
+enum NsPhase { GRAM, POLY, APPLY };
 
 struct NsProblem {
     int rows, cols, m, n, mp, np, batch;
@@ -43,32 +51,42 @@ struct NsProblem {
     int part, parts;                    // partial sums: first index, count per matrix
     float lr;
     int tiles;                          // of one matrix, in the launch at hand
+    int begin;                          // first tile of this entry, counted over the batch
+    int splits;                         // blocks that share a tile's summed index (1: none)
+    int slab;                           // first of their partial tiles in the slab
 };
 struct NsTable {
     int count;
+    int whole;                          // blocks that own a whole tile; the split ones follow
     int first[kMaxProblems + 1];        // first block of each problem, in the launch at hand
     NsProblem p[kMaxProblems];
 };
-static_assert(sizeof(NsTable) <= 3800, "kernel arguments");
+static_assert(sizeof(NsTable) <= 3900, "kernel arguments");
 
-// Workspace of one matrix: Y twice (this step's and the next one's) as [mp, np] planes and as
-// [np, mp] planes, the off-diagonal parts of A and B as [mp, mp] planes, their diagonals.
+// Row pitch of a plane: an odd number of 128-byte lines, so that the rows of a tile spread over the
+// memory channels (with a power of two they all meet in a few).
+__host__ __device__ inline int ns_pitch(int padded) { return (padded / 64) % 2 ? padded : padded + 64; }
+
+// Workspace of one matrix: Y twice (this step's and the next one's) as [mp, np] planes, the
+// off-diagonal parts of A and B as [mp, mp] planes, their diagonals.
 struct NsPlanes {
-    uint16_t *y, *yt, *o, *p;           // hi plane; the lo plane follows it
+    uint16_t *y, *o, *p;                // hi plane; the lo plane follows it
     float *d, *e;
-    size_t yplane, aplane;
+    size_t yplane, aplane;              // elements of a plane
+    int yld, ald;                       // pitches
 };
-__host__ __device__ inline size_t ns_matrix_bytes(size_t mp, size_t np) {
-    return 16 * mp * np + 8 * mp * mp + 8 * mp;
+inline size_t ns_matrix_bytes(int mp, int np) {
+    return 8 * (size_t)mp * ns_pitch(np) + 8 * (size_t)mp * ns_pitch(mp) + 8 * (size_t)mp;
 }
 __device__ __forceinline__ NsPlanes ns_planes(const NsProblem& q, char* ws, int b, int buffer) {
     NsPlanes r;
     uint16_t* base = (uint16_t*)(ws + q.ws + (size_t)b * q.ws_stride);
-    r.yplane = (size_t)q.mp * q.np;
-    r.aplane = (size_t)q.mp * q.mp;
+    r.yld = ns_pitch(q.np);
+    r.ald = ns_pitch(q.mp);
+    r.yplane = (size_t)q.mp * r.yld;
+    r.aplane = (size_t)q.mp * r.ald;
     r.y = base + (size_t)buffer * 2 * r.yplane;
-    r.yt = base + (size_t)(4 + buffer * 2) * r.yplane;
-    r.o = base + 8 * r.yplane;
+    r.o = base + 4 * r.yplane;
     r.p = r.o + 2 * r.aplane;
     r.d = (float*)(r.p + 2 * r.aplane);
     r.e = r.d + q.mp;
@@ -117,14 +135,29 @@ struct NsSegments {
     NsSegment s[64];
 };
 
-// The update direction of one element (its momentum already updated).
-__device__ __forceinline__ float ns_direction(const NsUpdate& u, long long at) {
-    const float m = u.m[at];
-    return u.nesterov ? u.g[at] * u.grad_scale + u.mu * m : m;
+// Eight consecutive elements as floats; `wide`: the address is a multiple of the vector's size.
+template <typename T>
+__device__ __forceinline__ void ns_load8(const T* p, bool wide, float (&v)[8]) {
+    if (wide) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = ((const float4*)p)[0], b = ((const float4*)p)[1];
+            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        } else {
+            const uint4 a = *(const uint4*)p;
+            const T* e = (const T*)&a;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = ns_elem(e[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = ns_elem(p[j]);
+    }
 }
 
-// Partial sums of squares in 64 bits: squares of fp32 values neither overflow nor vanish there.
-// A block takes 64 x 256 tiles.  In the update it first moves the momentum on.
+// Partial sums of squares in 64 bits: squares of fp32 values neither overflow nor vanish there.  A
+// wave takes 2048 consecutive elements of a row at a time, and a matrix without gaps between its
+// rows is one long row; 16-byte loads wherever the addresses allow them.  In the update the same
+// pass moves the momentum on.  Memory-bound.
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, const T* __restrict__ x, NsUpdate u,
                                                       double* __restrict__ partials) {
@@ -133,27 +166,57 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, const T* __re
     const NsProblem& q = tab.p[i];
     const int local = blockIdx.x - tab.first[i];
     const int b = local / q.parts, part = local % q.parts;
-    const int tiles_c = (q.cols + 255) / 256;
-    const long long tiles = (long long)((q.rows + 63) / 64) * tiles_c;
+    const bool flat = q.ld == q.cols;
+    const long long cols = flat ? (long long)q.rows * q.cols : q.cols;
+    const long long per_row = (cols + 2047) / 2048, units = per_row * (flat ? 1 : q.rows);
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     double sum = 0.0;
-    for (long long t = part; t < tiles; t += q.parts) {
-        const int r0 = (int)(t / tiles_c) * 64, c0 = (int)(t % tiles_c) * 256;
-        for (int r = r0 + wave; r < r0 + 64 && r < q.rows; r += 4) {
-            const long long row = q.src + b * q.stride + r * q.ld;
+    for (long long t = (long long)part * 4 + wave; t < units; t += (long long)q.parts * 4) {
+        const long long r = flat ? 0 : t / per_row;
+        const long long c0 = (flat ? t : t % per_row) * 2048;
+        const long long at0 = q.src + b * q.stride + r * q.ld + c0;
+        const bool full = c0 + 2048 <= cols;
+        if constexpr (MUON) {
+            if (full && (at0 & 3) == 0) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const long long at = at0 + k * 256 + lane * 4;
+                    const float4 g4 = *(const float4*)(u.g + at);
+                    float4 m4 = *(const float4*)(u.m + at);
+                    float v4[4];
+                    const float* g = (const float*)&g4;
+                    float* m = (float*)&m4;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float gj = g[j] * u.grad_scale;
+                        m[j] = u.mu * m[j] + gj;
+                        v4[j] = u.nesterov ? gj + u.mu * m[j] : m[j];
+                    }
+                    *(float4*)(u.m + at) = m4;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum += (double)v4[j] * (double)v4[j];
+                }
+            } else {
+                for (int k = lane; k < 2048 && c0 + k < cols; k += 64) {
+                    const float g = u.g[at0 + k] * u.grad_scale;
+                    const float m = u.mu * u.m[at0 + k] + g;
+                    u.m[at0 + k] = m;
+                    const float v = u.nesterov ? g + u.mu * m : m;
+                    sum += (double)v * (double)v;
+                }
+            }
+        } else if (full) {
+            const bool wide = ((uintptr_t)(x + at0) & 15) == 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const int c = c0 + k * 64 + lane;
-                if (c >= q.cols) continue;
-                float v;
-                if constexpr (MUON) {
-                    const float g = u.g[row + c] * u.grad_scale;
-                    const float m = u.mu * u.m[row + c] + g;
-                    u.m[row + c] = m;
-                    v = u.nesterov ? g + u.mu * m : m;
-                } else {
-                    v = ns_elem(x[row + c]);
-                }
+                float v[8];
+                ns_load8(x + at0 + k * 512 + lane * 8, wide, v);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum += (double)v[j] * (double)v[j];
+            }
+        } else {
+            for (int k = lane; k < 2048 && c0 + k < cols; k += 64) {
+                const float v = ns_elem(x[at0 + k]);
                 sum += (double)v * (double)v;
             }
         }
@@ -162,8 +225,8 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, const T* __re
     if (threadIdx.x == 0) partials[q.part + (size_t)b * q.parts + part] = sum;
 }
 
-// Y_0 = X / (||X|| + eps) as planes in both orientations, zeros in the padding.  64 x 64 tiles of
-// the matrix in memory, transposed through LDS.
+// Y_0 = X / (||X|| + eps) as planes, zeros in the padding.  64 x 64 tiles of the matrix in memory,
+// transposed through LDS where Y is its transpose.
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ns_load_kernel(NsTable tab, const T* __restrict__ x, NsUpdate u,
                                                       const double* __restrict__ partials, char* ws,
@@ -178,39 +241,71 @@ __global__ __launch_bounds__(256) void ns_load_kernel(NsTable tab, const T* __re
     for (int k = threadIdx.x; k < q.parts; k += 256) sum += partials[q.part + (size_t)b * q.parts + k];
     const double inv = (double)scale / (sqrt(block_sum(sum, smem)) + eps);
 
-    const int colsp = q.trans ? q.mp : q.np;
-    const int tiles_c = colsp / 64;
+    const int tiles_c = (q.trans ? q.mp : q.np) / 64;
     const int r0 = (t / tiles_c) * 64, c0 = (t % tiles_c) * 64;
-    for (int k = threadIdx.x; k < 4096; k += 256) {
-        const int r = r0 + (k >> 6), c = c0 + (k & 63);
-        float v = 0.f;
-        if (r < q.rows && c < q.cols) {
-            const long long at = q.src + b * q.stride + r * q.ld + c;
-            if constexpr (MUON) v = ns_direction(u, at);
-            else v = ns_elem(x[at]);
-            v = (float)((double)v * inv);
-        }
-        tile[k >> 6][k & 63] = v;
-    }
-    __syncthreads();
     const NsPlanes w = ns_planes(q, ws, b, 0);
-    // `same` has the orientation of the memory matrix, `flip` the other one
-    uint16_t* same = q.trans ? w.yt : w.y;
-    uint16_t* flip = q.trans ? w.y : w.yt;
-    const size_t same_ld = q.trans ? q.mp : q.np, flip_ld = q.trans ? q.np : q.mp;
+    const long long at0 = q.src + b * q.stride + (long long)r0 * q.ld + c0;
+    const bool full = r0 + 64 <= q.rows && c0 + 64 <= q.cols;
+#pragma unroll
+    for (int k = threadIdx.x; k < 512; k += 256) {
+        const int r = k >> 3, c = (k & 7) * 8;
+        const long long at = at0 + r * q.ld + c;
+        float v[8];
+        if (full) {
+            if constexpr (MUON) {
+                const bool wide = (at & 3) == 0;
+                float m[8];
+                ns_load8(u.m + at, wide, m);
+                if (u.nesterov) {
+                    ns_load8(u.g + at, wide, v);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = v[j] * u.grad_scale + u.mu * m[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[j] = m[j];
+                }
+            } else {
+                ns_load8(x + at, ((uintptr_t)(x + at) & 15) == 0, v);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = 0.f;
+                if (r0 + r < q.rows && c0 + c + j < q.cols) {
+                    if constexpr (MUON) {
+                        const float m = u.m[at + j];
+                        v[j] = u.nesterov ? u.g[at + j] * u.grad_scale + u.mu * m : m;
+                    } else {
+                        v[j] = ns_elem(x[at + j]);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)((double)v[j] * inv);
+        if (q.trans) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) tile[r][c + j] = v[j];
+        } else {
+            uint16_t hi[8], lo[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) split_f16(v[j], hi[j], lo[j]);
+            const size_t to = (size_t)(r0 + r) * w.yld + c0 + c;
+            *(uint4*)(w.y + to) = *(const uint4*)hi;
+            *(uint4*)(w.y + w.yplane + to) = *(const uint4*)lo;
+        }
+    }
+    if (!q.trans) return;
+    __syncthreads();
+#pragma unroll
     for (int k = threadIdx.x; k < 512; k += 256) {
         const int r = k >> 3, c = (k & 7) * 8;
         uint16_t hi[8], lo[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) split_f16(tile[r][c + j], hi[j], lo[j]);
-        const size_t at = (size_t)(r0 + r) * same_ld + c0 + c;
-        *(uint4*)(same + at) = *(const uint4*)hi;
-        *(uint4*)(same + w.yplane + at) = *(const uint4*)lo;
-#pragma unroll
         for (int j = 0; j < 8; ++j) split_f16(tile[c + j][r], hi[j], lo[j]);
-        const size_t ft = (size_t)(c0 + r) * flip_ld + r0 + c;
-        *(uint4*)(flip + ft) = *(const uint4*)hi;
-        *(uint4*)(flip + w.yplane + ft) = *(const uint4*)lo;
+        const size_t to = (size_t)(c0 + r) * w.yld + r0 + c;
+        *(uint4*)(w.y + to) = *(const uint4*)hi;
+        *(uint4*)(w.y + w.yplane + to) = *(const uint4*)lo;
     }
 }
 
@@ -229,7 +324,112 @@ __global__ __launch_bounds__(256) void ns_segments_kernel(NsSegments segs, float
     }
 }
 
-enum NsPhase { GRAM, POLY, APPLY };
+// Tile shapes of the products.  Tall: the summed index is long or the tiles are many.
+struct BigTile {        // 8 waves of 64 x 64, one block per CU, two stages in flight
+    static constexpr int kM = 128, kN = 256, kWavesM = 2, kWavesN = 4, kStages = 3, kBlocksPerCu = 1;
+};
+struct SmallTile {      // 4 waves of 32 x 32, two blocks per CU, three stages in flight
+    static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 4, kBlocksPerCu = 2;
+};
+
+// This wave's loads but the last N have landed and its LDS reads are done, then so for all waves.
+template <int N>
+__device__ __forceinline__ void await_stage() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+// Where the 32-byte pair p of a row of COLS fp16 with summed index k lies: at p ^ pair_swizzle(k).
+template <int COLS>
+__device__ __forceinline__ int pair_swizzle(int k) {
+    if (COLS >= 128) return (k & 3) | ((k >> 1) & 4);
+    return ((k >> 1) & 1) | ((k >> 2) & 2);         // two rows share the banks' 256 bytes
+}
+// Consecutive blocks go to the 8 XCDs in turn; with this numbering each XCD gets consecutive tiles,
+// which share rows of an operand in its L2.
+__device__ __forceinline__ int xcd_order(int block, int blocks) {
+    const int each = blocks >> 3, rest = blocks & 7, x = block & 7;
+    return x * each + (x < rest ? x : rest) + (block >> 3);
+}
+
+// Fragments of an operand that runs across the summed index: for each of FN column groups (LDS address
+// at[y]) the rows OFFSET bytes on and the rows STRIDE bytes further.  The reads and the wait for them
+// are one block of assembly: the compiler would put a wait for ALL loads in flight before the builtin,
+// since it cannot tell the stage that is read from those that are being filled.
+template <int FN, int OFFSET, int STRIDE>
+__device__ __forceinline__ void read_across(const unsigned (&at)[FN], f16x8 (&out)[FN]) {
+    static_assert(FN == 2 || FN == 4, "column groups");
+    f16x4 a[FN], b[FN];
+    if constexpr (FN == 4) {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+            "ds_read_b64_tr_b16 %1, %9 offset:%12\n\tds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+            "ds_read_b64_tr_b16 %2, %10 offset:%12\n\tds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+            "ds_read_b64_tr_b16 %3, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(a[0]), "=&v"(a[1]), "=&v"(a[2]), "=&v"(a[3]), "=&v"(b[0]), "=&v"(b[1]), "=&v"(b[2]),
+              "=&v"(b[3])
+            : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFFSET), "n"(OFFSET + STRIDE)
+            : "memory");
+    } else {
+        asm volatile(
+            "ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %2, %4 offset:%7\n\t"
+            "ds_read_b64_tr_b16 %1, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+            "s_waitcnt lgkmcnt(0)"
+            : "=&v"(a[0]), "=&v"(a[1]), "=&v"(b[0]), "=&v"(b[1])
+            : "v"(at[0]), "v"(at[1]), "n"(OFFSET), "n"(OFFSET + STRIDE)
+            : "memory");
+    }
+#pragma unroll
+    for (int y = 0; y < FN; ++y)
+        out[y] = f16x8{a[y][0], a[y][1], a[y][2], a[y][3], b[y][0], b[y][1], b[y][2], b[y][3]};
+}
+
+struct NsItem {
+    int problem, b, ti, tj, split, slab;     // split < 0: the block owns the tile
+};
+
+// Tiles of the symmetric products: those that touch the upper triangle, column by column.  A column
+// of tiles is kN / kM as wide as it is high, so column j has kN / kM * (j + 1) of them.
+template <typename G>
+__host__ __device__ inline int triangle_tiles(int mp) {
+    constexpr int R = G::kN / G::kM;
+    const int rows = (mp + G::kM - 1) / G::kM, cols = (mp + G::kN - 1) / G::kN;
+    return R * cols * (cols - 1) / 2 + rows;
+}
+template <typename G, int PHASE>
+__device__ __forceinline__ void tile_of(const NsProblem& q, int t, int& ti, int& tj) {
+    if (PHASE == APPLY) {
+        // groups of eight tile rows, column by column: neighbours share both operands
+        const int rows = (q.mp + G::kM - 1) / G::kM, cols = (q.np + G::kN - 1) / G::kN;
+        const int g = t / (8 * cols), in = t - g * 8 * cols;
+        const int high = rows - g * 8 < 8 ? rows - g * 8 : 8;
+        tj = in / high;
+        ti = g * 8 + in % high;
+    } else {
+        constexpr int R = G::kN / G::kM;
+        tj = 0;
+        while (R * (tj + 1) * (tj + 2) / 2 <= t) ++tj;
+        ti = t - R * tj * (tj + 1) / 2;
+    }
+}
+template <typename G, int PHASE>
+__device__ __forceinline__ NsItem item_of(const NsTable& tab, int block, int blocks) {
+    NsItem it;
+    const bool whole = block < tab.whole;
+    const int id = whole ? xcd_order(block, tab.whole) : tab.whole + xcd_order(block - tab.whole, blocks - tab.whole);
+    it.problem = ns_find(tab, id);
+    const NsProblem& q = tab.p[it.problem];
+    int local = id - tab.first[it.problem];
+    it.split = -1;
+    if (q.splits > 1) {
+        it.split = local % q.splits;
+        it.slab = q.slab + local;
+        local /= q.splits;
+    }
+    local += q.begin;
+    it.b = local / q.tiles;
+    tile_of<G, PHASE>(q, local % q.tiles, it.ti, it.tj);
+    return it;
+}
 
 struct NsStep {
     float a, b, c;
@@ -244,215 +444,344 @@ struct NsResult {
     float lr, decay;            // decay = 1 - lr * weight decay
 };
 
-// One T x T tile of a product of two matrices whose rows both run along the summed index.  The
-// four waves own quarters of the tile; 64 fp16 of every row are staged per step, either 64
-// consecutive hi values (narrow) or 32 hi and the same 32 lo values (wide), straight from memory
-// into LDS.  16-byte pieces of a row sit at (piece ^ (row & 7)), which spreads a fragment read
-// (16 rows, same piece) over the banks.
-template <int T, bool WIDE, int PHASE, typename OUT>
-__global__ __launch_bounds__(256, 2) void ns_product_kernel(NsTable tab, char* ws, NsStep s, NsResult res) {
-    constexpr int W = T / 2, N = W / 16;            // wave tile, fragments per side
-    constexpr int kStage = 2 * T * 128;
-    constexpr int kEld = T + 4;
-    constexpr int kSmem = 2 * kStage > T * kEld * 4 ? 2 * kStage : T * kEld * 4;
-    __shared__ __attribute__((aligned(1024))) char smem[kSmem];
+__device__ __forceinline__ void store_planes(uint16_t* hi_plane, size_t plane, const float (&z)[8]) {
+    uint16_t hi[8], lo[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) split_f16(z[j], hi[j], lo[j]);
+    *(uint4*)hi_plane = *(const uint4*)hi;
+    *(uint4*)(hi_plane + plane) = *(const uint4*)lo;
+}
+__device__ __forceinline__ void load_planes(const uint16_t* hi_plane, size_t plane, float (&z)[8]) {
+    const uint4 h4 = *(const uint4*)hi_plane, l4 = *(const uint4*)(hi_plane + plane);
+    const uint16_t *hi = (const uint16_t*)&h4, *lo = (const uint16_t*)&l4;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) z[j] = f16_value(hi[j]) + f16_value(lo[j]);
+}
 
-    const int i = ns_find(tab, blockIdx.x);
-    const NsProblem& q = tab.p[i];
-    const int local = blockIdx.x - tab.first[i];
-    const int b = local / q.tiles;
-    int t = local % q.tiles, ti, tj;
-    if (PHASE == APPLY) {
-        const int tiles_n = (q.np + T - 1) / T;
-        ti = t / tiles_n;
-        tj = t % tiles_n;
-    } else {        // upper triangle, row by row
-        const int tiles_m = (q.mp + T - 1) / T;
-        ti = 0;
-        while (t >= tiles_m - ti) { t -= tiles_m - ti; ++ti; }
-        tj = ti + t;
-    }
+// What follows a product: E holds M x N of its values in LDS (row pitch LD), from row i0, column j0.
+template <int M, int N, int LD, int THREADS, int BLOCK, int PHASE, typename OUT>
+__device__ __forceinline__ void ns_epilogue(float* E, const NsProblem& q, char* ws, int b, int i0, int j0,
+                                            const NsStep& s, const NsResult& res) {
     const NsPlanes w = ns_planes(q, ws, b, s.buffer);
-    const uint16_t *ah, *al, *bh, *bl;
-    int ld, depth, rows_b;
-    if (PHASE == GRAM) {
-        ah = bh = w.y; al = bl = w.y + w.yplane; ld = depth = q.np; rows_b = q.mp;
-    } else if (PHASE == POLY) {
-        ah = bh = w.o; al = bl = w.o + w.aplane; ld = depth = q.mp; rows_b = q.mp;
-    } else {
-        ah = w.p; al = w.p + w.aplane; bh = w.yt; bl = w.yt + w.yplane; ld = depth = q.mp; rows_b = q.np;
-    }
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int i0 = ti * T, j0 = tj * T;
-
-    auto stage = [&](int k0, int buf) {
-        char* dst = smem + buf * kStage;
-        const int piece = (lane & 7) ^ (lane >> 3);
-        const int kk = WIDE ? k0 + (piece & 3) * 8 : k0 + piece * 8;
-#pragma unroll
-        for (int r = wave * 8; r < T; r += 32) {
-            const int ra = i0 + r + (lane >> 3), rb = j0 + r + (lane >> 3);
-            const uint16_t* pa = (WIDE && piece >= 4 ? al : ah) + (size_t)(ra < q.mp ? ra : q.mp - 1) * ld + kk;
-            const uint16_t* pb = (WIDE && piece >= 4 ? bl : bh) + (size_t)(rb < rows_b ? rb : rows_b - 1) * ld + kk;
-            __builtin_amdgcn_global_load_lds((global_ptr)pa, (lds_ptr)(dst + r * 128), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((global_ptr)pb, (lds_ptr)(dst + T * 128 + r * 128), 16, 0, 0);
-        }
-    };
-
-    f32x4 acc[N][N];
-#pragma unroll
-    for (int x = 0; x < N; ++x)
-#pragma unroll
-        for (int y = 0; y < N; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-    const int wi = (wave >> 1) * W, wj = (wave & 1) * W;
-    const int l15 = lane & 15, lq = lane >> 4;
-    constexpr int kStep = WIDE ? 32 : 64;
-    const int steps = depth / kStep;
-    stage(0, 0);
-    for (int k = 0; k < steps; ++k) {
-        __syncthreads();
-        if (k + 1 < steps) stage((k + 1) * kStep, (k + 1) & 1);
-        const char* sa = smem + (k & 1) * kStage;
-        const char* sb = sa + T * 128;
-        f16x8 fa[2][N], fb[2][N];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int x = 0; x < N; ++x) {
-                const int ra = wi + x * 16 + l15, rb = wj + x * 16 + l15;
-                fa[h][x] = *(const f16x8*)(sa + ra * 128 + (((h * 4 + lq) ^ (ra & 7)) * 16));
-                fb[h][x] = *(const f16x8*)(sb + rb * 128 + (((h * 4 + lq) ^ (rb & 7)) * 16));
-            }
-#pragma unroll
-        for (int x = 0; x < N; ++x)
-#pragma unroll
-            for (int y = 0; y < N; ++y) {
-                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0][x], fb[0][y], acc[x][y], 0, 0, 0);
-                if (WIDE) {
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[0][x], fb[1][y], acc[x][y], 0, 0, 0);
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[1][x], fb[0][y], acc[x][y], 0, 0, 0);
-                } else {
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fa[1][x], fb[1][y], acc[x][y], 0, 0, 0);
-                }
-            }
-    }
-    __syncthreads();
-    float* E = (float*)smem;
-#pragma unroll
-    for (int x = 0; x < N; ++x)
-#pragma unroll
-        for (int y = 0; y < N; ++y)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                E[(wi + x * 16 + lq * 4 + r) * kEld + wj + y * 16 + l15] = acc[x][y][r] * s.inv;
-    __syncthreads();
-
+    constexpr int kVec = N / 8;
     if (PHASE == APPLY) {
-        const NsPlanes nx = ns_planes(q, ws, b, s.buffer ^ 1);
-        for (int v = threadIdx.x; v < T * T / 8; v += 256) {
-            const int r = v / (T / 8), c = (v % (T / 8)) * 8;
-            const int gi = i0 + r, gj = j0 + c;
-            if (gi >= q.mp || gj >= q.np) continue;
-            const float k = s.a + w.e[gi];
-            const size_t at = (size_t)gi * q.np + gj;
-            uint16_t hi[8], lo[8];
-            *(uint4*)hi = *(const uint4*)(w.y + at);
-            *(uint4*)lo = *(const uint4*)(w.y + w.yplane + at);
-            float z[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                z[j] = k * ((f16_value(hi[j]) + f16_value(lo[j])) / s.sx) + E[r * kEld + c + j];
-                E[r * kEld + c + j] = z[j];
-            }
-            if (!s.last) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) split_f16(z[j] * s.sx, hi[j], lo[j]);
-                *(uint4*)(nx.y + at) = *(const uint4*)hi;
-                *(uint4*)(nx.y + nx.yplane + at) = *(const uint4*)lo;
-            }
-        }
-        __syncthreads();
+        const float un = 1.f / s.sx;
         if (!s.last) {
-            for (int v = threadIdx.x; v < T * T / 8; v += 256) {
-                const int c = v / (T / 8), r = (v % (T / 8)) * 8;
-                const int gi = i0 + r, gj = j0 + c;
+            uint16_t* next = ns_planes(q, ws, b, s.buffer ^ 1).y;
+            for (int v = threadIdx.x; v < M * kVec; v += THREADS) {
+                const int r = v / kVec, c = (v % kVec) * 8, gi = i0 + r, gj = j0 + c;
                 if (gi >= q.mp || gj >= q.np) continue;
-                uint16_t hi[8], lo[8];
+                const float k = s.a + w.e[gi];
+                const size_t at = (size_t)gi * w.yld + gj;
+                float z[8];
+                load_planes(w.y + at, w.yplane, z);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) split_f16(E[(r + j) * kEld + c] * s.sx, hi[j], lo[j]);
-                const size_t at = (size_t)gj * q.mp + gi;
-                *(uint4*)(nx.yt + at) = *(const uint4*)hi;
-                *(uint4*)(nx.yt + nx.yplane + at) = *(const uint4*)lo;
+                for (int j = 0; j < 8; ++j) z[j] = k * z[j] + E[r * LD + c + j] * s.sx;
+                store_planes(next + at, w.yplane, z);
             }
             return;
         }
-        for (int v = threadIdx.x; v < T * T; v += 256) {
-            // consecutive threads along the rows of the matrix in memory
-            const int r = q.trans ? v % T : v / T, c = q.trans ? v / T : v % T;
-            const int gi = i0 + r, gj = j0 + c;
+        for (int v = threadIdx.x; v < M * kVec; v += THREADS) {
+            const int r = v / kVec, c = (v % kVec) * 8, gi = i0 + r, gj = j0 + c;
+            if (gi >= q.mp || gj >= q.np) continue;
+            const float k = s.a + w.e[gi];
+            float z[8];
+            load_planes(w.y + (size_t)gi * w.yld + gj, w.yplane, z);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = k * (z[j] * un) + E[r * LD + c + j];
+            if (q.trans) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) E[r * LD + c + j] = z[j];
+                continue;
+            }
             if (gi >= q.m || gj >= q.n) continue;
-            const float z = E[r * kEld + c];
-            const long long row = q.trans ? gj : gi, col = q.trans ? gi : gj;
+            const int have = q.n - gj;
             if (res.p) {
-                float* at = res.p + q.src + b * q.stride + row * q.ld + col;
+                float* at = res.p + q.src + b * q.stride + gi * q.ld + gj;
+                const float lr = res.lr * q.lr;
+                if (have >= 8 && ((uintptr_t)at & 15) == 0) {
+                    float4 p0 = ((float4*)at)[0], p1 = ((float4*)at)[1];
+                    p0.x = res.decay * p0.x - lr * z[0]; p0.y = res.decay * p0.y - lr * z[1];
+                    p0.z = res.decay * p0.z - lr * z[2]; p0.w = res.decay * p0.w - lr * z[3];
+                    p1.x = res.decay * p1.x - lr * z[4]; p1.y = res.decay * p1.y - lr * z[5];
+                    p1.z = res.decay * p1.z - lr * z[6]; p1.w = res.decay * p1.w - lr * z[7];
+                    ((float4*)at)[0] = p0;
+                    ((float4*)at)[1] = p1;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < have) at[j] = res.decay * at[j] - lr * z[j];
+                }
+            } else {
+                OUT* at = (OUT*)res.out + q.out + b * q.out_stride + gi * q.out_ld + gj;
+                OUT o[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = (OUT)z[j];
+                if (have >= 8 && ((uintptr_t)at & 15) == 0) {
+#pragma unroll
+                    for (int j = 0; j < (int)sizeof(o) / 16; ++j) ((uint4*)at)[j] = ((const uint4*)o)[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (j < have) at[j] = o[j];
+                }
+            }
+        }
+        if (!q.trans) return;
+        __syncthreads();
+        // consecutive threads along the rows of the matrix in memory, which are Y's columns
+        for (int v = threadIdx.x; v < M * N; v += THREADS) {
+            const int r = v % M, c = v / M, gi = i0 + r, gj = j0 + c;
+            if (gi >= q.m || gj >= q.n) continue;
+            const float z = E[r * LD + c];
+            if (res.p) {
+                float* at = res.p + q.src + b * q.stride + gj * q.ld + gi;
                 *at = res.decay * *at - res.lr * q.lr * z;
             } else {
-                ((OUT*)res.out)[q.out + b * q.out_stride + row * q.out_ld + col] = (OUT)z;
+                ((OUT*)res.out)[q.out + b * q.out_stride + gj * q.out_ld + gi] = (OUT)z;
             }
         }
         return;
     }
-
-    // GRAM: A = E.  POLY: A A = E + (d_i + d_j) O + [i = j] d_i^2, B = b A + c A A.
+    // GRAM: A = E.  POLY: A A = E + (d_i + d_j) O + [i = j] d_i^2, B = b A + c A A.  Squares of BLOCK
+    // above the diagonal are written twice, mirrored the second time; those below it not at all.
     uint16_t* dst = PHASE == GRAM ? w.o : w.p;
     float* diag = PHASE == GRAM ? w.d : w.e;
-    const float sc = PHASE == GRAM ? s.sa : s.sb;
-    for (int v = threadIdx.x; v < T * T / 8; v += 256) {
-        const int r = v / (T / 8), c = (v % (T / 8)) * 8;
-        const int gi = i0 + r, gj = j0 + c;
-        if (gi >= q.mp || gj >= q.mp) continue;
-        const size_t at = (size_t)gi * q.mp + gj;
-        uint16_t hi[8], lo[8];
+    const float sc = PHASE == GRAM ? s.sa : s.sb, un = 1.f / s.sa;
+    for (int v = threadIdx.x; v < M * kVec; v += THREADS) {
+        const int r = v / kVec, c = (v % kVec) * 8, gi = i0 + r, gj = j0 + c;
+        if (gi >= q.mp || gj >= q.mp || gj / BLOCK < gi / BLOCK) continue;
+        const size_t at = (size_t)gi * w.ald + gj;
+        float z[8], o[8];
         float di = 0.f;
         if (PHASE == POLY) {
-            *(uint4*)hi = *(const uint4*)(w.o + at);
-            *(uint4*)lo = *(const uint4*)(w.o + w.aplane + at);
+            load_planes(w.o + at, w.aplane, o);
             di = w.d[gi];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float z = E[r * kEld + c + j];
+            z[j] = E[r * LD + c + j];
             if (PHASE == POLY) {
-                const float dj = w.d[gj + j];
-                const float o = (f16_value(hi[j]) + f16_value(lo[j])) / s.sa;
-                z = gi == gj + j ? s.b * di + s.c * (z + di * di)
-                                 : s.b * o + s.c * (z + (di + dj) * o);
+                const float dj = w.d[gj + j], oj = o[j] * un;
+                z[j] = gi == gj + j ? s.b * di + s.c * (z[j] + di * di)
+                                    : s.b * oj + s.c * (z[j] + (di + dj) * oj);
             }
             if (gi == gj + j) {
-                diag[gi] = z;
-                z = 0.f;
+                diag[gi] = z[j];
+                z[j] = 0.f;
             }
-            z *= sc;
-            E[r * kEld + c + j] = z;
-            split_f16(z, hi[j], lo[j]);
+            z[j] *= sc;
+            E[r * LD + c + j] = z[j];
         }
-        *(uint4*)(dst + at) = *(const uint4*)hi;
-        *(uint4*)(dst + w.aplane + at) = *(const uint4*)lo;
+        store_planes(dst + at, w.aplane, z);
     }
-    if (ti == tj) return;
+    if ((j0 + N - 1) / BLOCK <= i0 / BLOCK) return;
     __syncthreads();
-    for (int v = threadIdx.x; v < T * T / 8; v += 256) {
-        const int c = v / (T / 8), r = (v % (T / 8)) * 8;
-        const int gi = i0 + r, gj = j0 + c;
-        if (gi >= q.mp || gj >= q.mp) continue;
-        const size_t at = (size_t)gj * q.mp + gi;
-        uint16_t hi[8], lo[8];
+    for (int v = threadIdx.x; v < M * N / 8; v += THREADS) {
+        const int c = v / (M / 8), r = (v % (M / 8)) * 8, gi = i0 + r, gj = j0 + c;
+        if (gi >= q.mp || gj >= q.mp || gj / BLOCK <= gi / BLOCK) continue;
+        float z[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) split_f16(E[(r + j) * kEld + c], hi[j], lo[j]);
-        *(uint4*)(dst + at) = *(const uint4*)hi;
-        *(uint4*)(dst + w.aplane + at) = *(const uint4*)lo;
+        for (int j = 0; j < 8; ++j) z[j] = E[(r + j) * LD + c];
+        store_planes(dst + (size_t)gj * w.ald + gi, w.aplane, z);
     }
+}
+
+// One tile of a product, or a part of its summed index.  64 fp16 of every row are staged per step,
+// either 64 consecutive hi values (narrow) or 32 hi and the same 32 lo values (wide), straight from
+// memory into a ring of LDS stages with counted waits and one barrier per step.
+//   * An operand whose rows run along the summed index: rows of 128 bytes, 16-byte piece p of row r at
+//     p ^ (r & 7), which spreads a fragment read (16 rows, same piece) over the banks.
+//   * Y in B Y runs across it: rows of one summed index, kN columns wide, read with the transposing
+//     LDS read (per 16 lanes a 4 x 16 block).  32-byte pair p of row k sits at p ^ pair_swizzle(k): the
+//     eight rows that half a wave reads at once meet different banks.
+// The columns' operand is the first of the MFMA, so a lane ends with four consecutive columns of a row.
+template <typename G, bool WIDE, int PHASE, typename OUT>
+__global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void ns_product_kernel(
+    NsTable tab, char* ws, float* slab, NsStep s, NsResult res) {
+    constexpr int kThreads = G::kWavesM * G::kWavesN * 64, kWaves = kThreads / 64;
+    constexpr int WM = G::kM / G::kWavesM, WN = G::kN / G::kWavesN, FM = WM / 16, FN = WN / 16;
+    constexpr int kStage = (G::kM + G::kN) * 128, LD = G::kN + 4;
+    constexpr int kRing = G::kStages * kStage, kTile = G::kM * LD * 4;
+    constexpr int kLoads = kStage / 1024 / kWaves;      // per wave and stage
+    constexpr int kStep = WIDE ? 32 : 64;
+    __shared__ __attribute__((aligned(1024))) char smem[kRing > kTile ? kRing : kTile];
+
+    const NsItem it = item_of<G, PHASE>(tab, blockIdx.x, gridDim.x);
+    const NsProblem& q = tab.p[it.problem];
+    const NsPlanes w = ns_planes(q, ws, it.b, s.buffer);
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int i0 = it.ti * G::kM, j0 = it.tj * G::kN;
+    // rows' operand, columns' operand
+    const uint16_t* rp = PHASE == GRAM ? w.y : PHASE == POLY ? w.o : w.p;
+    const uint16_t* cp = PHASE == POLY ? w.o : w.y;
+    const size_t rplane = PHASE == GRAM ? w.yplane : w.aplane, cplane = PHASE == POLY ? w.aplane : w.yplane;
+    const int rld = PHASE == GRAM ? w.yld : w.ald, cld = PHASE == POLY ? w.ald : w.yld;
+    const int depth = PHASE == GRAM ? q.np : q.mp;
+
+    int from = 0, to = depth / kStep;
+    if (it.split >= 0) {
+        const int all = to;
+        from = (int)((long long)all * it.split / q.splits);
+        to = (int)((long long)all * (it.split + 1) / q.splits);
+    }
+    const int steps = to - from;
+
+    // Addresses of this lane's pieces in the first stage; a stage on, they move by a fixed distance.
+    const char* src[kLoads];
+    long long hop[2];
+    hop[0] = kStep * 2;
+    hop[1] = PHASE == APPLY ? (long long)kStep * cld * 2 : kStep * 2;
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) {
+        const int kb = wave + l * kWaves;           // KB of the stage
+        if (kb < G::kM / 8) {
+            const int r = kb * 8 + (lane >> 3), piece = (lane & 7) ^ (lane >> 3);
+            int gi = i0 + r;
+            gi = gi < q.mp ? gi : q.mp - 1;
+            const int k = from * kStep + (WIDE ? (piece & 3) * 8 : piece * 8);
+            src[l] = (const char*)(rp + (WIDE && piece >= 4 ? rplane : 0) + (size_t)gi * rld + k);
+        } else if (PHASE != APPLY) {
+            const int r = (kb - G::kM / 8) * 8 + (lane >> 3), piece = (lane & 7) ^ (lane >> 3);
+            int gj = j0 + r;
+            gj = gj < q.mp ? gj : q.mp - 1;
+            const int k = from * kStep + (WIDE ? (piece & 3) * 8 : piece * 8);
+            src[l] = (const char*)(cp + (WIDE && piece >= 4 ? cplane : 0) + (size_t)gj * cld + k);
+        } else {
+            constexpr int kRowPieces = G::kN / 8;   // 16-byte pieces of a row
+            const int at = (kb - G::kM / 8) * 64 + lane;
+            const int row = at / kRowPieces, phys = at % kRowPieces;
+            const int k = WIDE ? row & 31 : row;
+            const int piece = phys ^ (pair_swizzle<G::kN>(k) * 2);
+            int gj = j0 + piece * 8;
+            gj = gj < q.np ? gj : q.np - 8;
+            src[l] = (const char*)(cp + (WIDE && row >= 32 ? cplane : 0) + (size_t)(from * kStep + k) * cld + gj);
+        }
+    }
+    auto stage = [&](int n) {
+        char* dst = smem + (n % G::kStages) * kStage;
+#pragma unroll
+        for (int l = 0; l < kLoads; ++l) {
+            const int kb = wave + l * kWaves;
+            __builtin_amdgcn_global_load_lds((global_ptr)src[l], (lds_ptr)(dst + kb * 1024), 16, 0, 0);
+            src[l] += kb < G::kM / 8 ? hop[0] : hop[1];
+        }
+    };
+
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int x = 0; x < FM; ++x)
+#pragma unroll
+        for (int y = 0; y < FN; ++y) acc[x][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const int wi = (wave / G::kWavesN) * WM, wj = (wave % G::kWavesN) * WN;
+    const int l15 = lane & 15, lq = lane >> 4;
+    unsigned across[FN];        // row lq*8 + l15/4, columns 4*(l15 & 3) of 16
+    if constexpr (PHASE == APPLY) {
+        const int row = lq * 8 + (l15 >> 2);
+#pragma unroll
+        for (int y = 0; y < FN; ++y) {
+            const int pair = ((wj + y * 16) >> 4) ^ pair_swizzle<G::kN>(row);
+            across[y] = (unsigned)(size_t)(lds_char*)smem + G::kM * 128 + row * (G::kN * 2) + pair * 32 + (l15 & 3) * 8;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < G::kStages - 1; ++n)
+        if (n < steps) stage(n);
+    for (int k = 0; k < steps; ++k) {
+        if (k + G::kStages - 2 < steps) await_stage<(G::kStages - 2) * kLoads>();
+        else await_stage<0>();
+        if (k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
+        const char* sr = smem + (k % G::kStages) * kStage;
+        const char* sc = sr + G::kM * 128;
+        f16x8 fr[2][FM], fc[2][FN];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int x = 0; x < FM; ++x) {
+                const int r = wi + x * 16 + l15;
+                fr[h][x] = *(const f16x8*)(sr + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
+            }
+#pragma unroll
+            for (int y = 0; y < FN; ++y) {
+                if constexpr (PHASE != APPLY) {
+                    const int r = wj + y * 16 + l15;
+                    fc[h][y] = *(const f16x8*)(sc + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
+                }
+            }
+        }
+        if constexpr (PHASE == APPLY) {
+            unsigned at[FN];
+#pragma unroll
+            for (int y = 0; y < FN; ++y) at[y] = across[y] + (unsigned)(k % G::kStages) * kStage;
+            read_across<FN, 0, 4 * G::kN * 2>(at, fc[0]);
+            read_across<FN, 32 * G::kN * 2, 4 * G::kN * 2>(at, fc[1]);
+        }
+#pragma unroll
+        for (int x = 0; x < FM; ++x)
+#pragma unroll
+            for (int y = 0; y < FN; ++y) {
+                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fc[0][y], fr[0][x], acc[x][y], 0, 0, 0);
+                if (WIDE) {
+                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fc[0][y], fr[1][x], acc[x][y], 0, 0, 0);
+                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fc[1][y], fr[0][x], acc[x][y], 0, 0, 0);
+                } else {
+                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fc[1][y], fr[1][x], acc[x][y], 0, 0, 0);
+                }
+            }
+    }
+    if (it.split >= 0) {        // fragments of 16 x 16, lane by lane
+        float* to_slab = slab + (size_t)it.slab * G::kM * G::kN;
+#pragma unroll
+        for (int x = 0; x < FM; ++x)
+#pragma unroll
+            for (int y = 0; y < FN; ++y)
+                *(f32x4*)(to_slab + ((size_t)((wi / 16 + x) * (G::kN / 16) + wj / 16 + y) * 64 + lane) * 4) = acc[x][y];
+        return;
+    }
+    __syncthreads();
+    float* E = (float*)smem;
+#pragma unroll
+    for (int x = 0; x < FM; ++x)
+#pragma unroll
+        for (int y = 0; y < FN; ++y)
+            *(f32x4*)(E + (wi + x * 16 + l15) * LD + wj + y * 16 + lq * 4) = acc[x][y] * s.inv;
+    __syncthreads();
+    ns_epilogue<G::kM, G::kN, LD, kThreads, G::kM, PHASE, OUT>(E, q, ws, it.b, i0, j0, s, res);
+}
+
+// Adds the parts of split tiles in the order of the summed index and finishes them, a 64 x 64 piece of
+// a tile per block.
+template <typename G, int PHASE, typename OUT>
+__global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, const float* __restrict__ slab,
+                                                      NsStep s, NsResult res) {
+    constexpr int kPieces = (G::kM / 64) * (G::kN / 64), LD = 68;
+    __shared__ float E[64 * LD];
+    const int id = blockIdx.x / kPieces, piece = blockIdx.x % kPieces;
+    const int p = ns_find(tab, id);
+    const NsProblem& q = tab.p[p];
+    const int local = id - tab.first[p];
+    const int b = (q.begin + local) / q.tiles;
+    int ti, tj;
+    tile_of<G, PHASE>(q, (q.begin + local) % q.tiles, ti, tj);
+    const int pi = (piece / (G::kN / 64)) * 64, pj = (piece % (G::kN / 64)) * 64;
+    const int i0 = ti * G::kM + pi, j0 = tj * G::kN + pj;
+    if (i0 >= q.mp || j0 >= (PHASE == APPLY ? q.np : q.mp)) return;
+    if (PHASE != APPLY && j0 / G::kM < i0 / G::kM) return;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lq = lane >> 4;
+    f32x4 sum[4];
+#pragma unroll
+    for (int y = 0; y < 4; ++y) sum[y] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const float* from = slab + (size_t)(q.slab + (size_t)local * q.splits) * G::kM * G::kN +
+                        ((size_t)((pi / 16 + wave) * (G::kN / 16) + pj / 16) * 64 + lane) * 4;
+    for (int k = 0; k < q.splits; ++k, from += G::kM * G::kN)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) sum[y] += *(const f32x4*)(from + y * 256);
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+        *(f32x4*)(E + (wave * 16 + l15) * LD + y * 16 + lq * 4) = sum[y] * s.inv;
+    __syncthreads();
+    ns_epilogue<64, 64, LD, 256, G::kM, PHASE, OUT>(E, q, ws, b, i0, j0, s, res);
 }
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
@@ -490,7 +819,137 @@ int scale_exp(double v) {
     return 15 - e;
 }
 
+// One launch: its table and how many blocks it takes.
+struct NsLaunch {
+    NsTable tab, join;          // `join`: the split entries, counted in tiles
+    unsigned blocks = 0, join_tiles = 0;
+    bool big = false;
+    size_t slab_bytes = 0;
+
+    static int checked(long long blocks) {
+        if (blocks > 0x3fffffffLL) throw std::invalid_argument("newton_schulz: too many blocks");
+        return (int)blocks;
+    }
+    template <typename F>
+    static NsLaunch simple(const std::vector<NsProblem>& ps, const F& blocks_of) {
+        NsLaunch l{};
+        long long at = 0;
+        for (const NsProblem& p : ps) {
+            NsProblem& e = l.tab.p[l.tab.count];
+            e = p;
+            e.tiles = checked(blocks_of(p));
+            l.tab.first[l.tab.count++] = checked(at);
+            at += blocks_of(p) * p.batch;
+        }
+        l.tab.first[l.tab.count] = checked(at);
+        l.blocks = (unsigned)at;
+        return l;
+    }
+
+    template <typename G>
+    static long long tiles_of(const NsProblem& p, int phase) {
+        if (phase != APPLY) return triangle_tiles<G>(p.mp);
+        return (long long)((p.mp + G::kM - 1) / G::kM) * ((p.np + G::kN - 1) / G::kN);
+    }
+    // Tiles fill the chip a round of kCus * kBlocksPerCu at a time.  Where they fill less than three
+    // quarters of the last round, its tiles' summed index is divided until they do.
+    template <typename G>
+    static NsLaunch tiled(const std::vector<NsProblem>& ps, int phase, bool wide, double& cost) {
+        constexpr int kSlots = kCus * G::kBlocksPerCu;
+        constexpr int kShortest = 8;        // steps below which a part costs more than it saves
+        const int step = wide ? 32 : 64;
+        NsLaunch l{};
+        struct Entry { NsProblem p; long long begin, count; int splits; };
+        std::vector<Entry> whole, split;
+        long long total = 0;
+        int longest = 0;
+        auto steps_of = [&](const NsProblem& p) { return (phase == GRAM ? p.np : p.mp) / step; };
+        for (const NsProblem& p : ps) {
+            total += checked(tiles_of<G>(p, phase)) * (long long)p.batch;
+            longest = std::max(longest, steps_of(p));
+        }
+        const long long rest = total % kSlots;
+        long long keep = total;         // tiles that stay whole
+        cost = 0;
+        if (rest && rest * 4 <= kSlots * 3) {
+            if (total < kSlots) {       // one round: parts of equal length, of all that are longer
+                int part = longest;
+                for (int n = kShortest; n < longest; ++n) {
+                    long long items = 0;
+                    for (const NsProblem& p : ps)
+                        items += tiles_of<G>(p, phase) * p.batch * ((steps_of(p) + n - 1) / n);
+                    if (items <= kSlots) { part = n; break; }
+                }
+                if (part + kShortest <= longest) {
+                    keep = 0;
+                    for (const NsProblem& p : ps) {
+                        const long long n = tiles_of<G>(p, phase) * p.batch;
+                        const int parts = (steps_of(p) + part - 1) / part;
+                        (parts > 1 ? split : whole).push_back({p, 0, n, parts});
+                    }
+                    cost = part + kShortest;
+                }
+            } else {
+                const int parts = (int)std::min<long long>(kSlots / rest, steps_of(ps.back()) / kShortest);
+                if (parts > 1) keep = total - rest;
+            }
+        }
+        if (keep) {
+            long long at = 0;
+            for (const NsProblem& p : ps) {
+                const long long n = tiles_of<G>(p, phase) * p.batch, w = std::max(0LL, std::min(n, keep - at));
+                if (w) whole.push_back({p, 0, w, 1});
+                if (w < n) {
+                    const int parts = (int)std::min<long long>(kSlots / rest, std::max(1, steps_of(p) / kShortest));
+                    (parts > 1 ? split : whole).push_back({p, w, n - w, parts});
+                }
+                at += n;
+            }
+            cost = (double)((keep + kSlots - 1) / kSlots) * longest;
+            if (keep < total) cost += kShortest + longest * (double)rest / kSlots;
+        }
+        long long at = 0, tiles = 0, slab = 0;
+        for (const std::vector<Entry>* list : {&whole, &split})
+            for (const Entry& e : *list) {
+                NsProblem& p = l.tab.p[l.tab.count];
+                p = e.p;
+                p.tiles = checked(tiles_of<G>(e.p, phase));
+                p.begin = checked(e.begin);
+                p.splits = e.splits;
+                p.slab = checked(slab);
+                l.tab.first[l.tab.count++] = checked(at);
+                at += e.count * e.splits;
+                if (list == &whole) {
+                    l.tab.whole = checked(at);
+                } else {
+                    slab += e.count * e.splits;
+                    l.join.p[l.join.count] = p;
+                    l.join.first[l.join.count++] = checked(tiles);
+                    tiles += e.count;
+                }
+            }
+        l.tab.first[l.tab.count] = l.blocks = (unsigned)checked(at);
+        l.join.first[l.join.count] = l.join_tiles = (unsigned)checked(tiles);
+        l.slab_bytes = (size_t)slab * G::kM * G::kN * sizeof(float);
+        return l;
+    }
+    static NsLaunch product(const std::vector<NsProblem>& ps, int phase, bool wide) {
+        double big_cost, small_cost;
+        NsLaunch big = tiled<BigTile>(ps, phase, wide, big_cost);
+        NsLaunch small = tiled<SmallTile>(ps, phase, wide, small_cost);
+        big.big = true;
+        const char* e = getenv("NS_TILE");
+        double f = e ? atof(e) : 3.0;
+        if (getenv("NS_DBG")) fprintf(stderr, "phase %d big cost %.1f blocks %u join %u small cost %.1f blocks %u join %u\n", phase, big_cost, big.blocks, big.join_tiles, small_cost, small.blocks, small.join_tiles);
+        return big_cost * f <= small_cost ? big : small;
+    }
+};
+
 }  // namespace
+
+struct NewtonSchulzPlan::Group {
+    NsLaunch norm, load, product[3];
+};
 
 NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
                                    const std::vector<NsSegment>& segments,
@@ -533,8 +992,46 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         at += (size_t)q.ws_stride * s.batch;
         mats_.push_back(q);
     }
-    for (const Matrix& q : mats_) at += (size_t)q.s.batch * kMaxPartials * sizeof(double);
-    ws_bytes_ = at;
+    // long sums first: a launch's last blocks are then its cheapest
+    std::vector<Matrix> order = mats_;
+    std::stable_sort(order.begin(), order.end(), [](const Matrix& x, const Matrix& y) { return x.np > y.np; });
+    long long partials = 0;
+    size_t slab = 0;
+    for (size_t lo = 0; lo < order.size(); lo += kMaxProblems - 1) {
+        groups_.push_back(std::make_shared<Group>());
+        Group& g = *groups_.back();
+        std::vector<NsProblem> ps;
+        for (size_t i = lo; i < std::min(lo + kMaxProblems - 1, order.size()); ++i) {
+            const Matrix& q = order[i];
+            NsProblem p{};
+            p.rows = q.s.rows; p.cols = q.s.cols; p.m = q.m; p.n = q.n; p.mp = q.mp; p.np = q.np;
+            p.batch = q.s.batch;
+            p.trans = q.s.rows > q.s.cols;
+            p.src = q.s.offset; p.ld = q.s.ld; p.stride = q.s.stride;
+            p.out = q.s.out_offset; p.out_ld = q.s.out_ld; p.out_stride = q.s.out_stride;
+            p.ws = q.ws; p.ws_stride = q.ws_stride;
+            p.lr = q.s.lr;
+            p.splits = 1;
+            const bool flat = p.ld == p.cols;
+            const long long cols = flat ? (long long)p.rows * p.cols : p.cols;
+            const long long units = (cols + 2047) / 2048 * (flat ? 1 : p.rows);
+            p.parts = (int)std::min<long long>((units + 3) / 4, kMaxPartials);
+            p.part = (int)partials;
+            partials += (long long)p.batch * p.parts;
+            if (partials > 0x7fffffffLL) throw std::invalid_argument("newton_schulz: too many matrices");
+            ps.push_back(p);
+        }
+        g.norm = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)p.parts; });
+        g.load = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)(p.mp / 64) * (p.np / 64); });
+        for (int phase : {(int)GRAM, (int)POLY, (int)APPLY}) {
+            g.product[phase] = NsLaunch::product(ps, phase, wide_);
+            slab = std::max(slab, g.product[phase].slab_bytes);
+        }
+    }
+    partials_ = at;
+    at += ((size_t)partials * sizeof(double) + 255) & ~(size_t)255;
+    slab_ = at;
+    ws_bytes_ = at + slab;
 }
 
 void NewtonSchulzPlan::check_workspace(const void* ws, size_t ws_bytes) const {
@@ -542,108 +1039,52 @@ void NewtonSchulzPlan::check_workspace(const void* ws, size_t ws_bytes) const {
         throw std::invalid_argument("newton_schulz: workspace too small or not 256-byte aligned");
 }
 
-// Up to kMaxProblems matrices of a plan and the table of the launch being made.
-struct NewtonSchulzPlan::Launch {
-    NsTable tab;
-    long long blocks = 0;
-    // `tiles(problem)`: blocks per matrix
-    template <typename F>
-    void count(const F& tiles) {
-        blocks = 0;
-        for (int i = 0; i < tab.count; ++i) {
-            tab.p[i].tiles = (int)tiles(tab.p[i]);
-            tab.first[i] = (int)blocks;
-            blocks += (long long)tiles(tab.p[i]) * tab.p[i].batch;
-            if (blocks > 0x7fffffffLL) throw std::invalid_argument("newton_schulz: too many blocks");
-        }
-        tab.first[tab.count] = (int)blocks;
-    }
-};
-
 namespace {
 
-template <int T, bool WIDE, typename OUT>
-void launch_phase(int phase, const NsTable& tab, unsigned blocks, char* ws, const NsStep& s,
-                  const NsResult& r, hipStream_t stream) {
-    if (phase == GRAM)
-        hipLaunchKernelGGL((ns_product_kernel<T, WIDE, GRAM, float>), dim3(blocks), dim3(256), 0, stream, tab, ws, s, r);
-    else if (phase == POLY)
-        hipLaunchKernelGGL((ns_product_kernel<T, WIDE, POLY, float>), dim3(blocks), dim3(256), 0, stream, tab, ws, s, r);
-    else
-        hipLaunchKernelGGL((ns_product_kernel<T, WIDE, APPLY, OUT>), dim3(blocks), dim3(256), 0, stream, tab, ws, s, r);
+template <typename G, bool WIDE, int PHASE, typename OUT>
+void launch_product(const NsLaunch& l, char* ws, float* slab, const NsStep& s, const NsResult& r,
+                    hipStream_t stream) {
+    hipLaunchKernelGGL((ns_product_kernel<G, WIDE, PHASE, OUT>), dim3(l.blocks),
+                       dim3(G::kWavesM * G::kWavesN * 64), 0, stream, l.tab, ws, slab, s, r);
+    if (l.join_tiles)
+        hipLaunchKernelGGL((ns_join_kernel<G, PHASE, OUT>), dim3(l.join_tiles * (G::kM / 64) * (G::kN / 64)),
+                           dim3(256), 0, stream, l.join, ws, slab, s, r);
 }
-template <int T>
-void launch_tile(bool wide, NsType type, int phase, const NsTable& tab, unsigned blocks, char* ws,
-                 const NsStep& s, const NsResult& r, hipStream_t stream) {
-    auto go = [&](auto w, auto out) {
-        launch_phase<T, decltype(w)::value, decltype(out)>(phase, tab, blocks, ws, s, r, stream);
-    };
-    auto pick = [&](auto w) {
-        if (type == NS_BF16) go(w, bf16_t{});
-        else if (type == NS_F16) go(w, f16_t{});
-        else go(w, 0.f);
-    };
-    if (wide) pick(std::true_type{});
-    else pick(std::false_type{});
+template <typename G, bool WIDE>
+void launch_phase(const NsLaunch& l, int phase, NsType type, char* ws, float* slab, const NsStep& s,
+                  const NsResult& r, hipStream_t stream) {
+    if (phase == GRAM) launch_product<G, WIDE, GRAM, float>(l, ws, slab, s, r, stream);
+    else if (phase == POLY) launch_product<G, WIDE, POLY, float>(l, ws, slab, s, r, stream);
+    else if (type == NS_BF16) launch_product<G, WIDE, APPLY, bf16_t>(l, ws, slab, s, r, stream);
+    else if (type == NS_F16) launch_product<G, WIDE, APPLY, f16_t>(l, ws, slab, s, r, stream);
+    else launch_product<G, WIDE, APPLY, float>(l, ws, slab, s, r, stream);
 }
 
 }  // namespace
 
-template <typename Prepare, typename Finish>
-void NewtonSchulzPlan::chain(void* ws_any, hipStream_t stream, const Prepare& prepare,
-                             const Finish& finish) const {
-    char* ws = (char*)ws_any;
-    size_t mat_bytes = 0;
-    for (const Matrix& q : mats_) mat_bytes = std::max(mat_bytes, (size_t)(q.ws + q.ws_stride * q.s.batch));
-    double* partials = (double*)(ws + mat_bytes);
-    for (size_t lo = 0; lo < mats_.size(); lo += kMaxProblems) {
-        Launch l;
-        NsTable& tab = l.tab;
-        tab.count = (int)std::min((size_t)kMaxProblems, mats_.size() - lo);
-        long long part = 0;
-        for (size_t i = 0; i < lo; ++i) part += (long long)mats_[i].s.batch * kMaxPartials;
-        for (int i = 0; i < tab.count; ++i) {
-            const Matrix& q = mats_[lo + i];
-            NsProblem& p = tab.p[i];
-            p.rows = q.s.rows; p.cols = q.s.cols; p.m = q.m; p.n = q.n; p.mp = q.mp; p.np = q.np;
-            p.batch = q.s.batch;
-            p.trans = q.s.rows > q.s.cols;
-            p.src = q.s.offset; p.ld = q.s.ld; p.stride = q.s.stride;
-            p.out = q.s.out_offset; p.out_ld = q.s.out_ld; p.out_stride = q.s.out_stride;
-            p.ws = q.ws; p.ws_stride = q.ws_stride;
-            const long long tiles = (long long)((p.rows + 63) / 64) * ((p.cols + 255) / 256);
-            p.parts = (int)std::min<long long>(tiles, kMaxPartials);
-            p.part = (int)part;
-            p.lr = q.s.lr;
-            part += (long long)p.batch * kMaxPartials;
-            if (part > 0x7fffffffLL) throw std::invalid_argument("newton_schulz: too many matrices");
-        }
-        l.count([](const NsProblem& p) { return (long long)p.parts; });
-        prepare(0, tab, (unsigned)l.blocks, partials, 0.f);
-        l.count([](const NsProblem& p) { return (long long)(p.mp / 64) * (p.np / 64); });
-        prepare(1, tab, (unsigned)l.blocks, partials, std::ldexp(1.f, x_exp_));
-
-        NsStep s;
-        s.sx = std::ldexp(1.f, x_exp_);
-        s.sa = std::ldexp(1.f, a_exp_);
-        s.sb = std::ldexp(1.f, b_exp_);
+template <typename Prepare>
+void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, void* out, float* p,
+                             float lr, float decay, hipStream_t stream) const {
+    NsResult r{out, p, lr, decay};
+    NsStep s{};
+    s.sx = std::ldexp(1.f, x_exp_);
+    s.sa = std::ldexp(1.f, a_exp_);
+    s.sb = std::ldexp(1.f, b_exp_);
+    float* slab = (float*)(ws + slab_);
+    for (const auto& g : groups_) {
+        prepare(*g, (double*)(ws + partials_), s.sx);
         const int steps = (int)coef_.size() / 3;
         for (int k = 0; k < steps; ++k) {
             s.a = coef_[3 * k]; s.b = coef_[3 * k + 1]; s.c = coef_[3 * k + 2];
             s.buffer = k & 1;
             s.last = k == steps - 1;
             for (int phase : {(int)GRAM, (int)POLY, (int)APPLY}) {
-                auto tiles_of = [&](int T) {
-                    return [T, phase](const NsProblem& p) {
-                        const long long tm = (p.mp + T - 1) / T, tn = (p.np + T - 1) / T;
-                        return phase == APPLY ? tm * tn : tm * (tm + 1) / 2;
-                    };
-                };
                 s.inv = std::ldexp(1.f, phase == GRAM ? -2 * x_exp_ : phase == POLY ? -2 * a_exp_ : -x_exp_ - b_exp_);
-                l.count(tiles_of(128));
-                const bool big = l.blocks >= 256;
-                if (!big) l.count(tiles_of(64));
-                finish(big, phase, tab, (unsigned)l.blocks, s);
+                const NsLaunch& l = g->product[phase];
+                if (l.big && wide_) launch_phase<BigTile, true>(l, phase, type, ws, slab, s, r, stream);
+                else if (l.big) launch_phase<BigTile, false>(l, phase, type, ws, slab, s, r, stream);
+                else if (wide_) launch_phase<SmallTile, true>(l, phase, type, ws, slab, s, r, stream);
+                else launch_phase<SmallTile, false>(l, phase, type, ws, slab, s, r, stream);
             }
         }
     }
@@ -654,31 +1095,26 @@ void NewtonSchulzPlan::orthogonalize(const void* x, void* out, NsType type, void
     if (mats_.empty()) return;
     check_workspace(ws, ws_bytes);
     if (!x || !out) throw std::invalid_argument("newton_schulz: null matrix");
-    auto prepare = [&](int pass, const NsTable& tab, unsigned blocks, double* partials, float scale) {
+    auto prepare = [&](const Group& g, double* partials, float scale) {
         auto go = [&](auto elem) {
             typedef decltype(elem) T;
-            if (pass == 0)
-                hipLaunchKernelGGL((ns_norm_kernel<T, false>), dim3(blocks), dim3(256), 0, stream, tab,
-                                   (const T*)x, NsUpdate{}, partials);
-            else
-                hipLaunchKernelGGL((ns_load_kernel<T, false>), dim3(blocks), dim3(256), 0, stream, tab,
-                                   (const T*)x, NsUpdate{}, partials, (char*)ws, eps_, scale);
+            hipLaunchKernelGGL((ns_norm_kernel<T, false>), dim3(g.norm.blocks), dim3(256), 0, stream,
+                               g.norm.tab, (const T*)x, NsUpdate{}, partials);
+            hipLaunchKernelGGL((ns_load_kernel<T, false>), dim3(g.load.blocks), dim3(256), 0, stream,
+                               g.load.tab, (const T*)x, NsUpdate{}, partials, (char*)ws, eps_, scale);
         };
         if (type == NS_BF16) go(bf16_t{});
         else if (type == NS_F16) go(f16_t{});
         else go(0.f);
     };
-    NsResult r{};
-    r.out = out;
-    chain(ws, stream, prepare, [&](bool big, int phase, const NsTable& tab, unsigned blocks, const NsStep& s) {
-        if (big) launch_tile<128>(wide_, type, phase, tab, blocks, (char*)ws, s, r, stream);
-        else launch_tile<64>(wide_, type, phase, tab, blocks, (char*)ws, s, r, stream);
-    });
+    chain((char*)ws, type, prepare, out, nullptr, 0.f, 0.f, stream);
 }
 
 void NewtonSchulzPlan::muon(float* p, const float* g, float* m, const MuonArgs& a, void* ws,
                             size_t ws_bytes, hipStream_t stream) const {
     if (!p || !g || !m) throw std::invalid_argument("muon: null buffer");
+    if (((uintptr_t)p | (uintptr_t)g | (uintptr_t)m) & 15)
+        throw std::invalid_argument("muon: buffers must be 16-byte aligned");
     check_workspace(ws, ws_bytes);
     for (size_t lo = 0; lo < segs_.size(); lo += 64) {
         NsSegments segs;
@@ -695,22 +1131,13 @@ void NewtonSchulzPlan::muon(float* p, const float* g, float* m, const MuonArgs& 
     }
     if (mats_.empty()) return;
     NsUpdate u{g, m, a.momentum, a.grad_scale, a.nesterov ? 1 : 0};
-    auto prepare = [&](int pass, const NsTable& tab, unsigned blocks, double* partials, float scale) {
-        if (pass == 0)
-            hipLaunchKernelGGL((ns_norm_kernel<float, true>), dim3(blocks), dim3(256), 0, stream, tab,
-                               (const float*)nullptr, u, partials);
-        else
-            hipLaunchKernelGGL((ns_load_kernel<float, true>), dim3(blocks), dim3(256), 0, stream, tab,
-                               (const float*)nullptr, u, partials, (char*)ws, eps_, scale);
+    auto prepare = [&](const Group& gr, double* partials, float scale) {
+        hipLaunchKernelGGL((ns_norm_kernel<float, true>), dim3(gr.norm.blocks), dim3(256), 0, stream,
+                           gr.norm.tab, (const float*)nullptr, u, partials);
+        hipLaunchKernelGGL((ns_load_kernel<float, true>), dim3(gr.load.blocks), dim3(256), 0, stream,
+                           gr.load.tab, (const float*)nullptr, u, partials, (char*)ws, eps_, scale);
     };
-    NsResult r{};
-    r.p = p;
-    r.lr = a.lr;
-    r.decay = 1.f - a.lr * a.weight_decay;
-    chain(ws, stream, prepare, [&](bool big, int phase, const NsTable& tab, unsigned blocks, const NsStep& s) {
-        if (big) launch_tile<128>(wide_, NS_F32, phase, tab, blocks, (char*)ws, s, r, stream);
-        else launch_tile<64>(wide_, NS_F32, phase, tab, blocks, (char*)ws, s, r, stream);
-    });
+    chain((char*)ws, NS_F32, prepare, nullptr, p, a.lr, 1.f - a.lr * a.weight_decay, stream);
 }
 
 }  // namespace dml

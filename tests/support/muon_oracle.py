@@ -29,7 +29,7 @@ def _planes(v, scale):
     return (hi + lo) / scale, hi / scale
 
 
-def modelled(x, wide, steps=5, coefficients=NS, eps=1e-7):
+def modelled(x, wide, steps=5, coefficients=NS, eps=1e-7, sums=None):
     """fp32 accumulation, planes of two fp16 terms (scaled by 2^13, a power of two that keeps every
     value of these tests in range), products of both terms (wide) or of the first (narrow), exact
     diagonals."""
@@ -48,6 +48,8 @@ def modelled(x, wide, steps=5, coefficients=NS, eps=1e-7):
         poly = b * (o + torch.diag(d)) + c * (f2 @ f2 + (d[:, None] + d[None, :]) * o + torch.diag(d * d))
         e = poly.diagonal().clone()
         p, ph = _planes(poly - torch.diag(e), 2.0 ** 12)
+        if sums is not None:
+            sums.append((abs(a), float((p.abs() @ y.abs()).norm()), y.shape[0]))
         y, yh = _planes((a + e)[:, None] * y + pick(p, ph) @ f, 2.0 ** 13)
     return y.T if x.shape[0] > x.shape[1] else y
 
@@ -66,7 +68,20 @@ def gradient(m, n, seed, batch=()):
 
 
 def tolerance(x, wide, out_dtype, **kw):
-    """Four times the rounding model's own error (accumulation order and the rare worse draw), plus
-    the rounding of the result: at most half a step per element."""
+    """Four times the rounding model's own error (the rare worse draw), the rounding of the sums that
+    the model does not share, and the rounding of the result: at most half a step per element.
+
+    Sums: the matrix units add 32 products at a time to an fp32 accumulator, for a wide product three
+    times, so an entry of P Y goes through n = 3 ceil(m / 32) roundings of at most 2^-24 of the partial
+    sum, itself at most (|P| |Y|)_ij; the model's own sums are blocked and round less often.  Unbiased
+    and independent, n of them come to sqrt(n) 2^-24 (|P| |Y|)_ij at most in the mean square, and four
+    times that covers the draw.  A difference in Y grows by at most |a| in each later step (the
+    polynomial's steepest slope), as it does where x has few directions: there the error is this term."""
     half_step = torch.finfo(out_dtype).eps / 2
-    return 4 * rel(modelled(x, wide, **kw), exact(x, **kw)) + half_step + 2.0 ** -22
+    sums, want = [], exact(x, **kw)
+    off = 4 * rel(modelled(x, wide, sums=sums, **kw), want)
+    grown = 0.0
+    for a, size, m in sums:
+        n = 3 * (-(-m // 32))
+        grown = a * grown + 4 * n ** 0.5 * 2.0 ** -24 * size
+    return off + grown / max(float(want.norm()), 1e-30) + half_step + 2.0 ** -22
