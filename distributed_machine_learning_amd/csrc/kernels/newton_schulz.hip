@@ -93,10 +93,12 @@ __device__ __forceinline__ NsPlanes ns_planes(const NsProblem& q, char* ws, int 
     return r;
 }
 
+// The problem a block works on: one load per lane and a vote instead of a chain of dependent loads.
+static_assert(kMaxProblems < 64, "one lane per problem");
 __device__ __forceinline__ int ns_find(const NsTable& t, int block) {
-    int i = 0;
-    while (i + 1 < t.count && block >= t.first[i + 1]) ++i;
-    return i;
+    const int lane = threadIdx.x & 63;
+    const bool past = lane < t.count && block >= t.first[lane];
+    return __popcll(__ballot(past)) - 1;
 }
 
 __device__ __forceinline__ uint16_t f16_bits(f16_t v) { return __builtin_bit_cast(uint16_t, v); }
@@ -327,15 +329,20 @@ __global__ __launch_bounds__(256) void ns_segments_kernel(NsSegments segs, float
 // Tile shapes of the products.  Tall: the summed index is long or the tiles are many.
 struct BigTile {        // 8 waves of 64 x 64, one block per CU, two stages in flight
     static constexpr int kM = 128, kN = 256, kWavesM = 2, kWavesN = 4, kStages = 3, kBlocksPerCu = 1;
+    static constexpr bool kTurns = true;
 };
 struct SmallTile {      // 4 waves of 32 x 32, two blocks per CU, three stages in flight
     static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 4, kBlocksPerCu = 2;
+    static constexpr bool kTurns = false;
 };
 
 // This wave's loads but the last N have landed and its LDS reads are done, then so for all waves.
 template <int N>
 __device__ __forceinline__ void await_stage() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void turn() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 // Where the 32-byte pair p of a row of COLS fp16 with summed index k lies: at p ^ pair_swizzle(k).
 template <int COLS>
@@ -451,42 +458,59 @@ __device__ __forceinline__ void store_planes(uint16_t* hi_plane, size_t plane, c
     *(uint4*)hi_plane = *(const uint4*)hi;
     *(uint4*)(hi_plane + plane) = *(const uint4*)lo;
 }
-__device__ __forceinline__ void load_planes(const uint16_t* hi_plane, size_t plane, float (&z)[8]) {
-    const uint4 h4 = *(const uint4*)hi_plane, l4 = *(const uint4*)(hi_plane + plane);
-    const uint16_t *hi = (const uint16_t*)&h4, *lo = (const uint16_t*)&l4;
+// What an epilogue reads: the planes of Y (APPLY) or O (POLY) under the tile, eight elements per
+// thread and turn.  All of it is requested at once, before the accumulators go to LDS: a turn at a
+// time would be a chain of memory latencies.
+template <int M, int N, int THREADS, int PHASE>
+struct NsOperand {
+    static constexpr int kVec = N / 8, kTurns = M * kVec / THREADS;
+    static_assert(M * kVec % THREADS == 0 && THREADS % kVec == 0, "whole turns");
+    uint4 hi[PHASE == GRAM ? 1 : kTurns], lo[PHASE == GRAM ? 1 : kTurns];
+
+    __device__ __forceinline__ void load(const NsProblem& q, const NsPlanes& w, int i0, int j0) {
+        if constexpr (PHASE != GRAM) {
+            const uint16_t* src = PHASE == APPLY ? w.y : w.o;
+            const size_t plane = PHASE == APPLY ? w.yplane : w.aplane;
+            const int ld = PHASE == APPLY ? w.yld : w.ald, cols = PHASE == APPLY ? q.np : q.mp;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) z[j] = f16_value(hi[j]) + f16_value(lo[j]);
-}
+            for (int n = 0; n < kTurns; ++n) {
+                const int v = threadIdx.x + n * THREADS, gi = i0 + v / kVec, gj = j0 + v % kVec * 8;
+                const bool in = gi < q.mp && gj < cols;
+                const uint16_t* at = src + (in ? (size_t)gi * ld + gj : 0);
+                hi[n] = *(const uint4*)at;
+                lo[n] = *(const uint4*)(at + plane);
+            }
+        }
+    }
+    __device__ __forceinline__ void value(int n, float (&z)[8]) const {
+        const uint16_t *h = (const uint16_t*)&hi[n], *l = (const uint16_t*)&lo[n];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] = f16_value(h[j]) + f16_value(l[j]);
+    }
+};
 
 // What follows a product: E holds M x N of its values in LDS (row pitch LD), from row i0, column j0.
 template <int M, int N, int LD, int THREADS, int BLOCK, int PHASE, typename OUT>
-__device__ __forceinline__ void ns_epilogue(float* E, const NsProblem& q, char* ws, int b, int i0, int j0,
-                                            const NsStep& s, const NsResult& res) {
-    const NsPlanes w = ns_planes(q, ws, b, s.buffer);
-    constexpr int kVec = N / 8;
-    if (PHASE == APPLY) {
+__device__ __forceinline__ void ns_epilogue(float* E, const NsOperand<M, N, THREADS, PHASE>& op,
+                                            const NsProblem& q, const NsPlanes& w, char* ws, int b, int i0,
+                                            int j0, const NsStep& s, const NsResult& res) {
+    constexpr int kVec = N / 8, kTurns = M * kVec / THREADS;
+    if constexpr (PHASE == APPLY) {
         const float un = 1.f / s.sx;
-        if (!s.last) {
-            uint16_t* next = ns_planes(q, ws, b, s.buffer ^ 1).y;
-            for (int v = threadIdx.x; v < M * kVec; v += THREADS) {
-                const int r = v / kVec, c = (v % kVec) * 8, gi = i0 + r, gj = j0 + c;
-                if (gi >= q.mp || gj >= q.np) continue;
-                const float k = s.a + w.e[gi];
-                const size_t at = (size_t)gi * w.yld + gj;
-                float z[8];
-                load_planes(w.y + at, w.yplane, z);
+        uint16_t* next = ns_planes(q, ws, b, s.buffer ^ 1).y;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) z[j] = k * z[j] + E[r * LD + c + j] * s.sx;
-                store_planes(next + at, w.yplane, z);
-            }
-            return;
-        }
-        for (int v = threadIdx.x; v < M * kVec; v += THREADS) {
-            const int r = v / kVec, c = (v % kVec) * 8, gi = i0 + r, gj = j0 + c;
+        for (int n = 0; n < kTurns; ++n) {
+            const int v = threadIdx.x + n * THREADS, r = v / kVec, c = v % kVec * 8, gi = i0 + r, gj = j0 + c;
             if (gi >= q.mp || gj >= q.np) continue;
             const float k = s.a + w.e[gi];
             float z[8];
-            load_planes(w.y + (size_t)gi * w.yld + gj, w.yplane, z);
+            op.value(n, z);
+            if (!s.last) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[j] = k * z[j] + E[r * LD + c + j] * s.sx;
+                store_planes(next + (size_t)gi * w.yld + gj, w.yplane, z);
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) z[j] = k * (z[j] * un) + E[r * LD + c + j];
             if (q.trans) {
@@ -527,7 +551,7 @@ __device__ __forceinline__ void ns_epilogue(float* E, const NsProblem& q, char* 
                 }
             }
         }
-        if (!q.trans) return;
+        if (!s.last || !q.trans) return;
         __syncthreads();
         // consecutive threads along the rows of the matrix in memory, which are Y's columns
         for (int v = threadIdx.x; v < M * N; v += THREADS) {
@@ -541,49 +565,52 @@ __device__ __forceinline__ void ns_epilogue(float* E, const NsProblem& q, char* 
                 ((OUT*)res.out)[q.out + b * q.out_stride + gj * q.out_ld + gi] = (OUT)z;
             }
         }
-        return;
-    }
-    // GRAM: A = E.  POLY: A A = E + (d_i + d_j) O + [i = j] d_i^2, B = b A + c A A.  Squares of BLOCK
-    // above the diagonal are written twice, mirrored the second time; those below it not at all.
-    uint16_t* dst = PHASE == GRAM ? w.o : w.p;
-    float* diag = PHASE == GRAM ? w.d : w.e;
-    const float sc = PHASE == GRAM ? s.sa : s.sb, un = 1.f / s.sa;
-    for (int v = threadIdx.x; v < M * kVec; v += THREADS) {
-        const int r = v / kVec, c = (v % kVec) * 8, gi = i0 + r, gj = j0 + c;
-        if (gi >= q.mp || gj >= q.mp || gj / BLOCK < gi / BLOCK) continue;
-        const size_t at = (size_t)gi * w.ald + gj;
-        float z[8], o[8];
-        float di = 0.f;
-        if (PHASE == POLY) {
-            load_planes(w.o + at, w.aplane, o);
-            di = w.d[gi];
-        }
+    } else {
+        // GRAM: A = E.  POLY: A A = E + (d_i + d_j) O + [i = j] d_i^2, B = b A + c A A.  Squares of BLOCK
+        // above the diagonal are written twice, mirrored the second time; those below it not at all.
+        uint16_t* dst = PHASE == GRAM ? w.o : w.p;
+        float* diag = PHASE == GRAM ? w.d : w.e;
+        const float sc = PHASE == GRAM ? s.sa : s.sb, un = 1.f / s.sa;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            z[j] = E[r * LD + c + j];
+        for (int n = 0; n < kTurns; ++n) {
+            const int v = threadIdx.x + n * THREADS, r = v / kVec, c = v % kVec * 8, gi = i0 + r, gj = j0 + c;
+            if (gi >= q.mp || gj >= q.mp || gj / BLOCK < gi / BLOCK) continue;
+            float z[8], o[8], dj[8];
+            float di = 0.f;
             if (PHASE == POLY) {
-                const float dj = w.d[gj + j], oj = o[j] * un;
-                z[j] = gi == gj + j ? s.b * di + s.c * (z[j] + di * di)
-                                    : s.b * oj + s.c * (z[j] + (di + dj) * oj);
+                op.value(n, o);
+                di = w.d[gi];
+                ns_load8(w.d + gj, true, dj);
             }
-            if (gi == gj + j) {
-                diag[gi] = z[j];
-                z[j] = 0.f;
-            }
-            z[j] *= sc;
-            E[r * LD + c + j] = z[j];
-        }
-        store_planes(dst + at, w.aplane, z);
-    }
-    if ((j0 + N - 1) / BLOCK <= i0 / BLOCK) return;
-    __syncthreads();
-    for (int v = threadIdx.x; v < M * N / 8; v += THREADS) {
-        const int c = v / (M / 8), r = (v % (M / 8)) * 8, gi = i0 + r, gj = j0 + c;
-        if (gi >= q.mp || gj >= q.mp || gj / BLOCK <= gi / BLOCK) continue;
-        float z[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] = E[(r + j) * LD + c];
-        store_planes(dst + (size_t)gj * w.ald + gi, w.aplane, z);
+            for (int j = 0; j < 8; ++j) {
+                z[j] = E[r * LD + c + j];
+                if (PHASE == POLY) {
+                    const float oj = o[j] * un;
+                    z[j] = gi == gj + j ? s.b * di + s.c * (z[j] + di * di)
+                                        : s.b * oj + s.c * (z[j] + (di + dj[j]) * oj);
+                }
+                if (gi == gj + j) {
+                    diag[gi] = z[j];
+                    z[j] = 0.f;
+                }
+                z[j] *= sc;
+                E[r * LD + c + j] = z[j];
+            }
+            store_planes(dst + (size_t)gi * w.ald + gj, w.aplane, z);
+        }
+        if ((j0 + N - 1) / BLOCK <= i0 / BLOCK) return;
+        __syncthreads();
+        // eight lanes to a row of 64 values, eight rows to a wave
+        for (int v = threadIdx.x; v < M * N / 8; v += THREADS) {
+            const int group = v >> 6, r = (group % (M / 64)) * 64 + (v & 7) * 8;
+            const int c = (group / (M / 64)) * 8 + (v >> 3 & 7), gi = i0 + r, gj = j0 + c;
+            if (gi >= q.mp || gj >= q.mp || gj / BLOCK <= gi / BLOCK) continue;
+            float z[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) z[j] = E[(r + j) * LD + c];
+            store_planes(dst + (size_t)gj * w.ald + gi, w.aplane, z);
+        }
     }
 }
 
@@ -688,47 +715,71 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
 #pragma unroll
     for (int n = 0; n < G::kStages - 1; ++n)
         if (n < steps) stage(n);
-    for (int k = 0; k < steps; ++k) {
-        if (k + G::kStages - 2 < steps) await_stage<(G::kStages - 2) * kLoads>();
-        else await_stage<0>();
-        if (k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
+    f16x8 fr[2][FM], fc[2][FN];
+    auto read = [&](int k) {
         const char* sr = smem + (k % G::kStages) * kStage;
-        const char* sc = sr + G::kM * 128;
-        f16x8 fr[2][FM], fc[2][FN];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int x = 0; x < FM; ++x) {
                 const int r = wi + x * 16 + l15;
                 fr[h][x] = *(const f16x8*)(sr + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
             }
-#pragma unroll
-            for (int y = 0; y < FN; ++y) {
-                if constexpr (PHASE != APPLY) {
-                    const int r = wj + y * 16 + l15;
-                    fc[h][y] = *(const f16x8*)(sc + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
-                }
-            }
-        }
         if constexpr (PHASE == APPLY) {
             unsigned at[FN];
 #pragma unroll
             for (int y = 0; y < FN; ++y) at[y] = across[y] + (unsigned)(k % G::kStages) * kStage;
             read_across<FN, 0, 4 * G::kN * 2>(at, fc[0]);
             read_across<FN, 32 * G::kN * 2, 4 * G::kN * 2>(at, fc[1]);
-        }
+        } else {
+            const char* sc = sr + G::kM * 128;
 #pragma unroll
-        for (int x = 0; x < FM; ++x)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int y = 0; y < FN; ++y) {
-                acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fc[0][y], fr[0][x], acc[x][y], 0, 0, 0);
-                if (WIDE) {
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fc[0][y], fr[1][x], acc[x][y], 0, 0, 0);
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fc[1][y], fr[0][x], acc[x][y], 0, 0, 0);
-                } else {
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fc[1][y], fr[1][x], acc[x][y], 0, 0, 0);
+                for (int y = 0; y < FN; ++y) {
+                    const int r = wj + y * 16 + l15;
+                    fc[h][y] = *(const f16x8*)(sc + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
                 }
-            }
+        }
+    };
+    auto multiply = [&]() {
+#pragma unroll
+        for (int n = 0; n < (WIDE ? 3 : 2); ++n)        // hi hi, hi lo, lo hi; or two halves of the step
+#pragma unroll
+            for (int x = 0; x < FM; ++x)
+#pragma unroll
+                for (int y = 0; y < FN; ++y)
+                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        fc[WIDE ? n >> 1 : n][y], fr[WIDE ? n & 1 : n][x], acc[x][y], 0, 0, 0);
+    };
+    auto await = [&](int k) {
+        if (k + G::kStages - 2 < steps) await_stage<(G::kStages - 2) * kLoads>();
+        else await_stage<0>();
+    };
+    if constexpr (G::kTurns) {
+        // The two waves of a SIMD take turns: half a step apart, one reads its fragments while the
+        // products of the other one run, and neither the LDS nor the matrix unit waits for the
+        // other.  The second half of the waves is one barrier behind; a stage has landed before the
+        // first half reads it and is refilled after the second half has.
+        const bool second = __builtin_amdgcn_readfirstlane(wave) >= kWaves / 2;
+        if (second) await(0);
+        for (int k = 0; k < steps; ++k) {
+            if (second) turn();
+            else await(k);
+            read(k);
+            if (k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
+            if (second) await(k + 1);
+            else turn();
+            multiply();
+        }
+        if (!second) turn();
+    } else {
+        for (int k = 0; k < steps; ++k) {
+            await(k);
+            if (k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
+            read(k);
+            multiply();
+        }
     }
     if (it.split >= 0) {        // fragments of 16 x 16, lane by lane
         float* to_slab = slab + (size_t)it.slab * G::kM * G::kN;
@@ -739,6 +790,8 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
                 *(f32x4*)(to_slab + ((size_t)((wi / 16 + x) * (G::kN / 16) + wj / 16 + y) * 64 + lane) * 4) = acc[x][y];
         return;
     }
+    NsOperand<G::kM, G::kN, kThreads, PHASE> op;
+    op.load(q, w, i0, j0);
     __syncthreads();
     float* E = (float*)smem;
 #pragma unroll
@@ -747,7 +800,7 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
         for (int y = 0; y < FN; ++y)
             *(f32x4*)(E + (wi + x * 16 + l15) * LD + wj + y * 16 + lq * 4) = acc[x][y] * s.inv;
     __syncthreads();
-    ns_epilogue<G::kM, G::kN, LD, kThreads, G::kM, PHASE, OUT>(E, q, ws, it.b, i0, j0, s, res);
+    ns_epilogue<G::kM, G::kN, LD, kThreads, G::kM, PHASE, OUT>(E, op, q, w, ws, it.b, i0, j0, s, res);
 }
 
 // Adds the parts of split tiles in the order of the summed index and finishes them, a 64 x 64 piece of
@@ -769,19 +822,34 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, con
     if (i0 >= q.mp || j0 >= (PHASE == APPLY ? q.np : q.mp)) return;
     if (PHASE != APPLY && j0 / G::kM < i0 / G::kM) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lq = lane >> 4;
+    const NsPlanes w = ns_planes(q, ws, b, s.buffer);
+    NsOperand<64, 64, 256, PHASE> op;
+    op.load(q, w, i0, j0);
     f32x4 sum[4];
 #pragma unroll
     for (int y = 0; y < 4; ++y) sum[y] = f32x4{0.f, 0.f, 0.f, 0.f};
     const float* from = slab + (size_t)(q.slab + (size_t)local * q.splits) * G::kM * G::kN +
                         ((size_t)((pi / 16 + wave) * (G::kN / 16) + pj / 16) * 64 + lane) * 4;
-    for (int k = 0; k < q.splits; ++k, from += G::kM * G::kN)
+    constexpr int kBatch = 8;       // parts in flight; one at a time is a chain of memory latencies
+    for (int k = 0; k < q.splits; k += kBatch) {
+        f32x4 part[kBatch][4];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) sum[y] += *(const f32x4*)(from + y * 256);
+        for (int n = 0; n < kBatch; ++n) {
+            const float* at = from + (size_t)(k + n < q.splits ? k + n : q.splits - 1) * G::kM * G::kN;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) part[n][y] = *(const f32x4*)(at + y * 256);
+        }
+#pragma unroll
+        for (int n = 0; n < kBatch; ++n)
+            if (k + n < q.splits)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sum[y] += part[n][y];
+    }
 #pragma unroll
     for (int y = 0; y < 4; ++y)
         *(f32x4*)(E + (wave * 16 + l15) * LD + y * 16 + lq * 4) = sum[y] * s.inv;
     __syncthreads();
-    ns_epilogue<64, 64, LD, 256, G::kM, PHASE, OUT>(E, q, ws, b, i0, j0, s, res);
+    ns_epilogue<64, 64, LD, 256, G::kM, PHASE, OUT>(E, op, q, w, ws, b, i0, j0, s, res);
 }
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
