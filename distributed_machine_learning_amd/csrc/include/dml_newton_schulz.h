@@ -63,6 +63,7 @@ class NewtonSchulzPlan {
         long long ws, ws_stride;     // workspace of the first matrix and between matrices, bytes
     };
     struct Group;                    // the launches of as many matrices as a launch takes
+    struct Op;                       // one product of the chain
     void check_workspace(const void* ws, size_t ws_bytes) const;
     template <typename Prepare>
     void chain(char* ws, NsType type, const Prepare& prepare, void* out, float* p, float lr, float decay,
@@ -72,8 +73,9 @@ class NewtonSchulzPlan {
     std::vector<NsSegment> segs_;
     std::vector<float> coef_;
     double eps_;
-    bool wide_;
-    int x_exp_, a_exp_, b_exp_;      // planes hold value * 2^exp
+    bool wide_, squares_wide_ = false;
+    int x_exp_;                      // Y's planes hold value * 2^exp
+    std::vector<std::shared_ptr<Op>> ops_;
     std::vector<std::shared_ptr<Group>> groups_;
     size_t partials_ = 0, slab_ = 0, ws_bytes_ = 0;      // offsets in the workspace, its size
 };

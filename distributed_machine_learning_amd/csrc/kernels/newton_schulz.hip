@@ -40,7 +40,8 @@ constexpr int kPad = 64;                // planes are zero-padded to multiples o
 constexpr int kMaxPartials = 1024;      // blocks (partial sums of squares) per matrix
 constexpr int kCus = 256;
 
-enum NsPhase { GRAM, POLY, APPLY };
+// Kinds of products: A = Y Y^T; Z = X W of two m x m polynomials in one A; Y <- P Y.
+enum NsPhase { GRAM, SQUARE, APPLY };
 
 struct NsProblem {
     int rows, cols, m, n, mp, np, batch;
@@ -67,29 +68,31 @@ static_assert(sizeof(NsTable) <= 3900, "kernel arguments");
 // memory channels (with a power of two they all meet in a few).
 __host__ __device__ inline int ns_pitch(int padded) { return (padded / 64) % 2 ? padded : padded + 64; }
 
-// Workspace of one matrix: Y twice (this step's and the next one's) as [mp, np] planes, the
-// off-diagonal parts of A and B as [mp, mp] planes, their diagonals.
+// Workspace of one matrix: Y twice (this product's and the next one's) as [mp, np] planes, the
+// diagonals of the [mp, mp] matrices and their off-diagonal parts as planes.  The hi plane comes first.
+constexpr int kSquares = 5;
 struct NsPlanes {
-    uint16_t *y, *o, *p;                // hi plane; the lo plane follows it
-    float *d, *e;
+    uint16_t *y, *squares;
+    float* diagonals;
     size_t yplane, aplane;              // elements of a plane
-    int yld, ald;                       // pitches
+    int yld, ald, mp;                   // pitches
+    __device__ __forceinline__ uint16_t* square(int i) const { return squares + (size_t)i * 2 * aplane; }
+    __device__ __forceinline__ float* diagonal(int i) const { return diagonals + i * mp; }
 };
-inline size_t ns_matrix_bytes(int mp, int np) {
-    return 8 * (size_t)mp * ns_pitch(np) + 8 * (size_t)mp * ns_pitch(mp) + 8 * (size_t)mp;
+inline size_t ns_matrix_bytes(int mp, int np, int squares) {
+    return 8 * (size_t)mp * ns_pitch(np) + 4 * kSquares * (size_t)mp + 4 * squares * (size_t)mp * ns_pitch(mp);
 }
 __device__ __forceinline__ NsPlanes ns_planes(const NsProblem& q, char* ws, int b, int buffer) {
     NsPlanes r;
     uint16_t* base = (uint16_t*)(ws + q.ws + (size_t)b * q.ws_stride);
+    r.mp = q.mp;
     r.yld = ns_pitch(q.np);
     r.ald = ns_pitch(q.mp);
     r.yplane = (size_t)q.mp * r.yld;
     r.aplane = (size_t)q.mp * r.ald;
     r.y = base + (size_t)buffer * 2 * r.yplane;
-    r.o = base + 4 * r.yplane;
-    r.p = r.o + 2 * r.aplane;
-    r.d = (float*)(r.p + 2 * r.aplane);
-    r.e = r.d + q.mp;
+    r.diagonals = (float*)(base + 4 * r.yplane);
+    r.squares = (uint16_t*)(r.diagonals + kSquares * q.mp);
     return r;
 }
 
@@ -330,10 +333,17 @@ __global__ __launch_bounds__(256) void ns_segments_kernel(NsSegments segs, float
 struct BigTile {        // 8 waves of 64 x 64, one block per CU, two stages in flight
     static constexpr int kM = 128, kN = 256, kWavesM = 2, kWavesN = 4, kStages = 3, kBlocksPerCu = 1;
     static constexpr bool kTurns = true;
+    static constexpr double kWideStep = 1.0, kNarrowStep = 0.85, kTileUs = 13;
+};
+struct MidTile {        // 4 waves of 64 x 64, two blocks per CU, one stage in flight
+    static constexpr int kM = 128, kN = 128, kWavesM = 2, kWavesN = 2, kStages = 2, kBlocksPerCu = 2;
+    static constexpr bool kTurns = false;
+    static constexpr double kWideStep = 1.4, kNarrowStep = 1.1, kTileUs = 8;
 };
 struct SmallTile {      // 4 waves of 32 x 32, two blocks per CU, three stages in flight
     static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 4, kBlocksPerCu = 2;
     static constexpr bool kTurns = false;
+    static constexpr double kWideStep = 0.5, kNarrowStep = 0.45, kTileUs = 4;
 };
 
 // This wave's loads but the last N have landed and its LDS reads are done, then so for all waves.
@@ -439,10 +449,12 @@ __device__ __forceinline__ NsItem item_of(const NsTable& tab, int block, int blo
 }
 
 struct NsStep {
-    float a, b, c;
-    float sx, sa, sb;           // plane scales 2^e
     float inv;                  // accumulator -> value
-    int buffer;                 // planes of this step's Y
+    float sy;                   // Y's planes hold value * sy
+    float ix, iw, sz;           // SQUARE: planes of X, W -> value; value -> planes of Z
+    float k0, k1, k2;           // SQUARE: Z = k0 + k1 X W + k2 W
+    int x, w, z;                // indices of the m x m matrices (GRAM writes z, APPLY multiplies by x)
+    int buffer;                 // planes of Y that are read
     int last;                   // APPLY: write the result instead of the next planes
 };
 struct NsResult {
@@ -458,28 +470,22 @@ __device__ __forceinline__ void store_planes(uint16_t* hi_plane, size_t plane, c
     *(uint4*)hi_plane = *(const uint4*)hi;
     *(uint4*)(hi_plane + plane) = *(const uint4*)lo;
 }
-// What an epilogue reads: the planes of Y (APPLY) or O (POLY) under the tile, eight elements per
-// thread and turn.  All of it is requested at once, before the accumulators go to LDS: a turn at a
-// time would be a chain of memory latencies.
-template <int M, int N, int THREADS, int PHASE>
+// Eight consecutive elements of a thread in each of its turns over a tile, requested all at once and
+// before the accumulators go to LDS.  Stores count as loads in flight, so a load between the stores of
+// two turns would wait for the first of them to reach memory (3300 clocks a turn instead of 500).
+template <int M, int N, int THREADS>
 struct NsOperand {
     static constexpr int kVec = N / 8, kTurns = M * kVec / THREADS;
     static_assert(M * kVec % THREADS == 0 && THREADS % kVec == 0, "whole turns");
-    uint4 hi[PHASE == GRAM ? 1 : kTurns], lo[PHASE == GRAM ? 1 : kTurns];
+    uint4 hi[kTurns], lo[kTurns];
 
-    __device__ __forceinline__ void load(const NsProblem& q, const NsPlanes& w, int i0, int j0) {
-        if constexpr (PHASE != GRAM) {
-            const uint16_t* src = PHASE == APPLY ? w.y : w.o;
-            const size_t plane = PHASE == APPLY ? w.yplane : w.aplane;
-            const int ld = PHASE == APPLY ? w.yld : w.ald, cols = PHASE == APPLY ? q.np : q.mp;
+    __device__ __forceinline__ void load(const uint16_t* src, size_t plane, int ld, int rows, int cols, int i0, int j0) {
 #pragma unroll
-            for (int n = 0; n < kTurns; ++n) {
-                const int v = threadIdx.x + n * THREADS, gi = i0 + v / kVec, gj = j0 + v % kVec * 8;
-                const bool in = gi < q.mp && gj < cols;
-                const uint16_t* at = src + (in ? (size_t)gi * ld + gj : 0);
-                hi[n] = *(const uint4*)at;
-                lo[n] = *(const uint4*)(at + plane);
-            }
+        for (int n = 0; n < kTurns; ++n) {
+            const int v = threadIdx.x + n * THREADS, gi = i0 + v / kVec, gj = j0 + v % kVec * 8;
+            const uint16_t* at = src + (gi < rows && gj < cols ? (size_t)gi * ld + gj : 0);
+            hi[n] = *(const uint4*)at;
+            lo[n] = *(const uint4*)(at + plane);
         }
     }
     __device__ __forceinline__ void value(int n, float (&z)[8]) const {
@@ -489,112 +495,120 @@ struct NsOperand {
     }
 };
 
-// What follows a product: E holds M x N of its values in LDS (row pitch LD), from row i0, column j0.
-template <int M, int N, int LD, int THREADS, int BLOCK, int PHASE, typename OUT>
-__device__ __forceinline__ void ns_epilogue(float* E, const NsOperand<M, N, THREADS, PHASE>& op,
-                                            const NsProblem& q, const NsPlanes& w, char* ws, int b, int i0,
-                                            int j0, const NsStep& s, const NsResult& res) {
+// What follows a product.  `put` writes the M x N values of the tile (accumulators times s.inv) to
+// E in LDS, row pitch LD; rows / cols hold the diagonals of the operands along the tile's sides; the
+// tile starts at row i0, column j0.
+template <int M, int N, int LD, int THREADS, int BLOCK, int PHASE, typename OUT, typename PUT>
+__device__ __forceinline__ void ns_epilogue(float* E, const float* rows, const float* cols, const NsProblem& q,
+                                            const NsPlanes& w, char* ws, int b, int i0, int j0, const NsStep& s,
+                                            const NsResult& res, const PUT& put) {
     constexpr int kVec = N / 8, kTurns = M * kVec / THREADS;
     if constexpr (PHASE == APPLY) {
-        const float un = 1.f / s.sx;
+        NsOperand<M, N, THREADS> y;
+        y.load(w.y, w.yplane, w.yld, q.mp, q.np, i0, j0);
+        put();
+        const float un = 1.f / s.sy;
         uint16_t* next = ns_planes(q, ws, b, s.buffer ^ 1).y;
+        if (!s.last) {
+#pragma unroll
+            for (int n = 0; n < kTurns; ++n) {
+                const int v = threadIdx.x + n * THREADS, r = v / kVec, c = v % kVec * 8, gi = i0 + r, gj = j0 + c;
+                if (gi >= q.mp || gj >= q.np) continue;
+                float z[8];
+                y.value(n, z);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) z[j] = rows[r] * z[j] + E[r * LD + c + j] * s.sy;
+                store_planes(next + (size_t)gi * w.yld + gj, w.yplane, z);
+            }
+            return;
+        }
 #pragma unroll
         for (int n = 0; n < kTurns; ++n) {
-            const int v = threadIdx.x + n * THREADS, r = v / kVec, c = v % kVec * 8, gi = i0 + r, gj = j0 + c;
-            if (gi >= q.mp || gj >= q.np) continue;
-            const float k = s.a + w.e[gi];
+            const int v = threadIdx.x + n * THREADS, r = v / kVec, c = v % kVec * 8;
             float z[8];
-            op.value(n, z);
-            if (!s.last) {
+            y.value(n, z);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) z[j] = k * z[j] + E[r * LD + c + j] * s.sx;
-                store_planes(next + (size_t)gi * w.yld + gj, w.yplane, z);
-                continue;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) z[j] = k * (z[j] * un) + E[r * LD + c + j];
-            if (q.trans) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) E[r * LD + c + j] = z[j];
-                continue;
-            }
-            if (gi >= q.m || gj >= q.n) continue;
-            const int have = q.n - gj;
-            if (res.p) {
-                float* at = res.p + q.src + b * q.stride + gi * q.ld + gj;
-                const float lr = res.lr * q.lr;
-                if (have >= 8 && ((uintptr_t)at & 15) == 0) {
-                    float4 p0 = ((float4*)at)[0], p1 = ((float4*)at)[1];
-                    p0.x = res.decay * p0.x - lr * z[0]; p0.y = res.decay * p0.y - lr * z[1];
-                    p0.z = res.decay * p0.z - lr * z[2]; p0.w = res.decay * p0.w - lr * z[3];
-                    p1.x = res.decay * p1.x - lr * z[4]; p1.y = res.decay * p1.y - lr * z[5];
-                    p1.z = res.decay * p1.z - lr * z[6]; p1.w = res.decay * p1.w - lr * z[7];
-                    ((float4*)at)[0] = p0;
-                    ((float4*)at)[1] = p1;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j < have) at[j] = res.decay * at[j] - lr * z[j];
-                }
-            } else {
-                OUT* at = (OUT*)res.out + q.out + b * q.out_stride + gi * q.out_ld + gj;
-                OUT o[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = (OUT)z[j];
-                if (have >= 8 && ((uintptr_t)at & 15) == 0) {
-#pragma unroll
-                    for (int j = 0; j < (int)sizeof(o) / 16; ++j) ((uint4*)at)[j] = ((const uint4*)o)[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j < have) at[j] = o[j];
-                }
-            }
+            for (int j = 0; j < 8; ++j) E[r * LD + c + j] += rows[r] * (z[j] * un);
         }
-        if (!s.last || !q.trans) return;
         __syncthreads();
-        // consecutive threads along the rows of the matrix in memory, which are Y's columns
-        for (int v = threadIdx.x; v < M * N; v += THREADS) {
-            const int r = v % M, c = v / M, gi = i0 + r, gj = j0 + c;
-            if (gi >= q.m || gj >= q.n) continue;
-            const float z = E[r * LD + c];
+        // Consecutive threads along the rows of the matrix in memory, four elements each; where Y is
+        // its transpose those are Y's columns.
+        const int wide = q.trans ? M : N;
+        const int rest = q.trans ? q.m - i0 : q.n - j0, deep = q.trans ? q.n - j0 : q.m - i0;
+        const long long ld = res.p ? q.ld : q.out_ld;
+        const long long base = (res.p ? q.src + b * q.stride : q.out + b * q.out_stride) +
+                               (q.trans ? (long long)j0 * ld + i0 : (long long)i0 * ld + j0);
+        const float lr = res.lr * q.lr;
+#pragma unroll 2
+        for (int v = threadIdx.x; v < M * N / 4; v += THREADS) {
+            const int c = v % (wide / 4) * 4, r = v / (wide / 4);
+            if (r >= deep || c >= rest) continue;
+            float z[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) z[j] = q.trans ? E[(c + j) * LD + r] : E[r * LD + c + j];
+            const long long to = base + r * ld + c;
+            const bool all = c + 4 <= rest;
             if (res.p) {
-                float* at = res.p + q.src + b * q.stride + gj * q.ld + gi;
-                *at = res.decay * *at - res.lr * q.lr * z;
+                float* at = res.p + to;
+                if (all && ((uintptr_t)at & 15) == 0) {
+                    float4 p4 = *(float4*)at;
+                    p4.x = res.decay * p4.x - lr * z[0];
+                    p4.y = res.decay * p4.y - lr * z[1];
+                    p4.z = res.decay * p4.z - lr * z[2];
+                    p4.w = res.decay * p4.w - lr * z[3];
+                    *(float4*)at = p4;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (c + j < rest) at[j] = res.decay * at[j] - lr * z[j];
+                }
             } else {
-                ((OUT*)res.out)[q.out + b * q.out_stride + gj * q.out_ld + gi] = (OUT)z;
+                struct alignas(4 * sizeof(OUT)) Four { OUT e[4]; } o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o.e[j] = (OUT)z[j];
+                OUT* at = (OUT*)res.out + to;
+                if (all && ((uintptr_t)at & (sizeof(Four) - 1)) == 0) {
+                    *(Four*)at = o;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (c + j < rest) at[j] = o.e[j];
+                }
             }
         }
     } else {
-        // GRAM: A = E.  POLY: A A = E + (d_i + d_j) O + [i = j] d_i^2, B = b A + c A A.  Squares of BLOCK
-        // above the diagonal are written twice, mirrored the second time; those below it not at all.
-        uint16_t* dst = PHASE == GRAM ? w.o : w.p;
-        float* diag = PHASE == GRAM ? w.d : w.e;
-        const float sc = PHASE == GRAM ? s.sa : s.sb, un = 1.f / s.sa;
+        // Squares of BLOCK above the diagonal are written twice, mirrored the second time; those below
+        // it not at all.
+        NsOperand<M, N, THREADS> ox, ow;
+        if constexpr (PHASE == SQUARE) {
+            ow.load(w.square(s.w), w.aplane, w.ald, q.mp, q.mp, i0, j0);
+            ox.load(w.square(s.x), w.aplane, w.ald, q.mp, q.mp, i0, j0);
+        }
+        put();
+        uint16_t* dst = w.square(s.z);
+        float* diag = w.diagonal(s.z);
 #pragma unroll
         for (int n = 0; n < kTurns; ++n) {
             const int v = threadIdx.x + n * THREADS, r = v / kVec, c = v % kVec * 8, gi = i0 + r, gj = j0 + c;
             if (gi >= q.mp || gj >= q.mp || gj / BLOCK < gi / BLOCK) continue;
-            float z[8], o[8], dj[8];
-            float di = 0.f;
-            if (PHASE == POLY) {
-                op.value(n, o);
-                di = w.d[gi];
-                ns_load8(w.d + gj, true, dj);
+            float z[8], x8[8], w8[8];
+            if (PHASE == SQUARE) {
+                ox.value(n, x8);
+                ow.value(n, w8);
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 z[j] = E[r * LD + c + j];
-                if (PHASE == POLY) {
-                    const float oj = o[j] * un;
-                    z[j] = gi == gj + j ? s.b * di + s.c * (z[j] + di * di)
-                                        : s.b * oj + s.c * (z[j] + (di + dj[j]) * oj);
+                if (PHASE == SQUARE) {
+                    const float dx = rows[r], dw = cols[c + j], o = w8[j] * s.iw;
+                    z[j] = gi == gj + j ? s.k1 * (z[j] + dx * dw) + (s.k2 * dw + s.k0)
+                                        : s.k1 * (z[j] + (dx * o + x8[j] * s.ix * dw)) + s.k2 * o;
                 }
                 if (gi == gj + j) {
                     diag[gi] = z[j];
                     z[j] = 0.f;
                 }
-                z[j] *= sc;
+                z[j] *= s.sz;
                 E[r * LD + c + j] = z[j];
             }
             store_planes(dst + (size_t)gi * w.ald + gj, w.aplane, z);
@@ -602,6 +616,7 @@ __device__ __forceinline__ void ns_epilogue(float* E, const NsOperand<M, N, THRE
         if ((j0 + N - 1) / BLOCK <= i0 / BLOCK) return;
         __syncthreads();
         // eight lanes to a row of 64 values, eight rows to a wave
+#pragma unroll 2
         for (int v = threadIdx.x; v < M * N / 8; v += THREADS) {
             const int group = v >> 6, r = (group % (M / 64)) * 64 + (v & 7) * 8;
             const int c = (group / (M / 64)) * 8 + (v >> 3 & 7), gi = i0 + r, gj = j0 + c;
@@ -613,6 +628,21 @@ __device__ __forceinline__ void ns_epilogue(float* E, const NsOperand<M, N, THRE
         }
     }
 }
+// The operands' diagonals along a tile's sides: requested first of all, put to LDS last of all.
+template <int M, int N, int PHASE>
+struct NsSides {
+    float row = 0.f, col = 0.f;
+    __device__ __forceinline__ void load(const NsPlanes& w, const NsStep& s, int i0, int j0) {
+        const int t = threadIdx.x;
+        if (PHASE != GRAM && t < M && i0 + t < w.mp) row = w.diagonal(s.x)[i0 + t];
+        if (PHASE == SQUARE && t < N && j0 + t < w.mp) col = w.diagonal(s.w)[j0 + t];
+    }
+    __device__ __forceinline__ void put(float* rows, float* cols) const {
+        const int t = threadIdx.x;
+        if (PHASE != GRAM && t < M) rows[t] = row;
+        if (PHASE == SQUARE && t < N) cols[t] = col;
+    }
+};
 
 // One tile of a product, or a part of its summed index.  64 fp16 of every row are staged per step,
 // either 64 consecutive hi values (narrow) or 32 hi and the same 32 lo values (wide), straight from
@@ -633,6 +663,8 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
     constexpr int kLoads = kStage / 1024 / kWaves;      // per wave and stage
     constexpr int kStep = WIDE ? 32 : 64;
     __shared__ __attribute__((aligned(1024))) char smem[kRing > kTile ? kRing : kTile];
+    __shared__ float rows[G::kM], cols[G::kN];
+    static_assert(kThreads >= G::kM && kThreads >= G::kN, "one thread per row and column");
 
     const NsItem it = item_of<G, PHASE>(tab, blockIdx.x, gridDim.x);
     const NsProblem& q = tab.p[it.problem];
@@ -640,11 +672,13 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int i0 = it.ti * G::kM, j0 = it.tj * G::kN;
     // rows' operand, columns' operand
-    const uint16_t* rp = PHASE == GRAM ? w.y : PHASE == POLY ? w.o : w.p;
-    const uint16_t* cp = PHASE == POLY ? w.o : w.y;
-    const size_t rplane = PHASE == GRAM ? w.yplane : w.aplane, cplane = PHASE == POLY ? w.aplane : w.yplane;
-    const int rld = PHASE == GRAM ? w.yld : w.ald, cld = PHASE == POLY ? w.ald : w.yld;
+    const uint16_t* rp = PHASE == GRAM ? w.y : w.square(s.x);
+    const uint16_t* cp = PHASE == SQUARE ? w.square(s.w) : w.y;
+    const size_t rplane = PHASE == GRAM ? w.yplane : w.aplane, cplane = PHASE == SQUARE ? w.aplane : w.yplane;
+    const int rld = PHASE == GRAM ? w.yld : w.ald, cld = PHASE == SQUARE ? w.ald : w.yld;
     const int depth = PHASE == GRAM ? q.np : q.mp;
+    NsSides<G::kM, G::kN, PHASE> sides;
+    sides.load(w, s, i0, j0);
 
     int from = 0, to = depth / kStep;
     if (it.split >= 0) {
@@ -790,17 +824,18 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
                 *(f32x4*)(to_slab + ((size_t)((wi / 16 + x) * (G::kN / 16) + wj / 16 + y) * 64 + lane) * 4) = acc[x][y];
         return;
     }
-    NsOperand<G::kM, G::kN, kThreads, PHASE> op;
-    op.load(q, w, i0, j0);
-    __syncthreads();
     float* E = (float*)smem;
+    auto put = [&]() {
+        sides.put(rows, cols);
+        __syncthreads();        // the ring's last stage has been read
 #pragma unroll
-    for (int x = 0; x < FM; ++x)
+        for (int x = 0; x < FM; ++x)
 #pragma unroll
-        for (int y = 0; y < FN; ++y)
-            *(f32x4*)(E + (wi + x * 16 + l15) * LD + wj + y * 16 + lq * 4) = acc[x][y] * s.inv;
-    __syncthreads();
-    ns_epilogue<G::kM, G::kN, LD, kThreads, G::kM, PHASE, OUT>(E, op, q, w, ws, it.b, i0, j0, s, res);
+            for (int y = 0; y < FN; ++y)
+                *(f32x4*)(E + (wi + x * 16 + l15) * LD + wj + y * 16 + lq * 4) = acc[x][y] * s.inv;
+        __syncthreads();
+    };
+    ns_epilogue<G::kM, G::kN, LD, kThreads, G::kM, PHASE, OUT>(E, rows, cols, q, w, ws, it.b, i0, j0, s, res, put);
 }
 
 // Adds the parts of split tiles in the order of the summed index and finishes them, a 64 x 64 piece of
@@ -809,7 +844,7 @@ template <typename G, int PHASE, typename OUT>
 __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, const float* __restrict__ slab,
                                                       NsStep s, NsResult res) {
     constexpr int kPieces = (G::kM / 64) * (G::kN / 64), LD = 68;
-    __shared__ float E[64 * LD];
+    __shared__ float E[64 * LD], rows[64], cols[64];
     const int id = blockIdx.x / kPieces, piece = blockIdx.x % kPieces;
     const int p = ns_find(tab, id);
     const NsProblem& q = tab.p[p];
@@ -823,33 +858,36 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, con
     if (PHASE != APPLY && j0 / G::kM < i0 / G::kM) return;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lq = lane >> 4;
     const NsPlanes w = ns_planes(q, ws, b, s.buffer);
-    NsOperand<64, 64, 256, PHASE> op;
-    op.load(q, w, i0, j0);
-    f32x4 sum[4];
+    NsSides<64, 64, PHASE> sides;
+    sides.load(w, s, i0, j0);
+    auto put = [&]() {
+        f32x4 sum[4];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) sum[y] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float* from = slab + (size_t)(q.slab + (size_t)local * q.splits) * G::kM * G::kN +
-                        ((size_t)((pi / 16 + wave) * (G::kN / 16) + pj / 16) * 64 + lane) * 4;
-    constexpr int kBatch = 8;       // parts in flight; one at a time is a chain of memory latencies
-    for (int k = 0; k < q.splits; k += kBatch) {
-        f32x4 part[kBatch][4];
+        for (int y = 0; y < 4; ++y) sum[y] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const float* from = slab + (size_t)(q.slab + (size_t)local * q.splits) * G::kM * G::kN +
+                            ((size_t)((pi / 16 + wave) * (G::kN / 16) + pj / 16) * 64 + lane) * 4;
+        constexpr int kBatch = 4;       // parts in flight; one at a time is a chain of memory latencies
+        for (int k = 0; k < q.splits; k += kBatch) {
+            f32x4 part[kBatch][4];
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n) {
-            const float* at = from + (size_t)(k + n < q.splits ? k + n : q.splits - 1) * G::kM * G::kN;
+            for (int n = 0; n < kBatch; ++n) {
+                const float* at = from + (size_t)(k + n < q.splits ? k + n : q.splits - 1) * G::kM * G::kN;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) part[n][y] = *(const f32x4*)(at + y * 256);
+                for (int y = 0; y < 4; ++y) part[n][y] = *(const f32x4*)(at + y * 256);
+            }
+#pragma unroll
+            for (int n = 0; n < kBatch; ++n)
+                if (k + n < q.splits)
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) sum[y] += part[n][y];
         }
+        sides.put(rows, cols);
 #pragma unroll
-        for (int n = 0; n < kBatch; ++n)
-            if (k + n < q.splits)
-#pragma unroll
-                for (int y = 0; y < 4; ++y) sum[y] += part[n][y];
-    }
-#pragma unroll
-    for (int y = 0; y < 4; ++y)
-        *(f32x4*)(E + (wave * 16 + l15) * LD + y * 16 + lq * 4) = sum[y] * s.inv;
-    __syncthreads();
-    ns_epilogue<64, 64, LD, 256, G::kM, PHASE, OUT>(E, op, q, w, ws, b, i0, j0, s, res);
+        for (int y = 0; y < 4; ++y)
+            *(f32x4*)(E + (wave * 16 + l15) * LD + y * 16 + lq * 4) = sum[y] * s.inv;
+        __syncthreads();
+    };
+    ns_epilogue<64, 64, LD, 256, G::kM, PHASE, OUT>(E, rows, cols, q, w, ws, b, i0, j0, s, res, put);
 }
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
@@ -871,12 +909,12 @@ double poly_max(double a, double b, double c, double r) {
     }
     return best;
 }
-// Largest |b z + c z^2| over [0, r].
-double poly2_max(double b, double c, double r) {
-    double best = std::fabs(r * (b + c * r));
+// Largest |a + b z + c z^2| over [0, r].
+double factor_max(double a, double b, double c, double r) {
+    double best = std::max(std::fabs(a), std::fabs(a + r * (b + c * r)));
     if (c != 0.0) {
         const double z = -b / (2 * c);
-        if (z > 0 && z < r) best = std::max(best, std::fabs(z * (b + c * z)));
+        if (z > 0 && z < r) best = std::max(best, std::fabs(a + z * (b + c * z)));
     }
     return best;
 }
@@ -891,7 +929,7 @@ int scale_exp(double v) {
 struct NsLaunch {
     NsTable tab, join;          // `join`: the split entries, counted in tiles
     unsigned blocks = 0, join_tiles = 0;
-    bool big = false;
+    int tile = 0;               // 0 big, 1 mid, 2 small
     size_t slab_bytes = 0;
 
     static int checked(long long blocks) {
@@ -920,11 +958,13 @@ struct NsLaunch {
         return (long long)((p.mp + G::kM - 1) / G::kM) * ((p.np + G::kN - 1) / G::kN);
     }
     // Tiles fill the chip a round of kCus * kBlocksPerCu at a time.  Where they fill less than three
-    // quarters of the last round, its tiles' summed index is divided until they do.
+    // quarters of the last round, its tiles' summed index may be divided until they do; whether it is
+    // goes by the estimate `cost` in microseconds (the tile shapes' measured constants).
     template <typename G>
     static NsLaunch tiled(const std::vector<NsProblem>& ps, int phase, bool wide, double& cost) {
         constexpr int kSlots = kCus * G::kBlocksPerCu;
-        constexpr int kShortest = 8;        // steps below which a part costs more than it saves
+        constexpr int kShortest = 4;            // steps of the shortest part
+        const double step_us = wide ? G::kWideStep : G::kNarrowStep;
         const int step = wide ? 32 : 64;
         NsLaunch l{};
         struct Entry { NsProblem p; long long begin, count; int splits; };
@@ -936,30 +976,40 @@ struct NsLaunch {
             total += checked(tiles_of<G>(p, phase)) * (long long)p.batch;
             longest = std::max(longest, steps_of(p));
         }
-        const long long rest = total % kSlots;
+        auto join_us = [&](long long items) { return 7.0 + (double)items * G::kM * G::kN * 8 / 4e6; };
+        const long long rest = total % kSlots, rounds = (total + kSlots - 1) / kSlots;
         long long keep = total;         // tiles that stay whole
-        cost = 0;
+        cost = rounds * (longest * step_us + G::kTileUs);
         if (rest && rest * 4 <= kSlots * 3) {
             if (total < kSlots) {       // one round: parts of equal length, of all that are longer
                 int part = longest;
+                long long items = total;
                 for (int n = kShortest; n < longest; ++n) {
-                    long long items = 0;
+                    items = 0;
                     for (const NsProblem& p : ps)
                         items += tiles_of<G>(p, phase) * p.batch * ((steps_of(p) + n - 1) / n);
                     if (items <= kSlots) { part = n; break; }
                 }
-                if (part + kShortest <= longest) {
+                const double divided = part * step_us + 0.5 * G::kTileUs + join_us(items);
+                if (part < longest && divided < cost) {
+                    cost = divided;
                     keep = 0;
                     for (const NsProblem& p : ps) {
                         const long long n = tiles_of<G>(p, phase) * p.batch;
                         const int parts = (steps_of(p) + part - 1) / part;
                         (parts > 1 ? split : whole).push_back({p, 0, n, parts});
                     }
-                    cost = part + kShortest;
                 }
             } else {
                 const int parts = (int)std::min<long long>(kSlots / rest, steps_of(ps.back()) / kShortest);
-                if (parts > 1) keep = total - rest;
+                if (parts > 1) {
+                    const double divided = (rounds - 1) * (longest * step_us + G::kTileUs) +
+                                           (double)longest / parts * step_us + 0.5 * G::kTileUs + join_us(rest * parts);
+                    if (divided < cost) {
+                        cost = divided;
+                        keep = total - rest;
+                    }
+                }
             }
         }
         if (keep) {
@@ -973,8 +1023,6 @@ struct NsLaunch {
                 }
                 at += n;
             }
-            cost = (double)((keep + kSlots - 1) / kSlots) * longest;
-            if (keep < total) cost += kShortest + longest * (double)rest / kSlots;
         }
         long long at = 0, tiles = 0, slab = 0;
         for (const std::vector<Entry>* list : {&whole, &split})
@@ -1002,14 +1050,17 @@ struct NsLaunch {
         return l;
     }
     static NsLaunch product(const std::vector<NsProblem>& ps, int phase, bool wide) {
-        double big_cost, small_cost;
-        NsLaunch big = tiled<BigTile>(ps, phase, wide, big_cost);
-        NsLaunch small = tiled<SmallTile>(ps, phase, wide, small_cost);
-        big.big = true;
-        const char* e = getenv("NS_TILE");
-        double f = e ? atof(e) : 3.0;
-        if (getenv("NS_DBG")) fprintf(stderr, "phase %d big cost %.1f blocks %u join %u small cost %.1f blocks %u join %u\n", phase, big_cost, big.blocks, big.join_tiles, small_cost, small.blocks, small.join_tiles);
-        return big_cost * f <= small_cost ? big : small;
+        double cost[3];
+        NsLaunch l[3] = {tiled<BigTile>(ps, phase, wide, cost[0]), tiled<MidTile>(ps, phase, wide, cost[1]),
+                         tiled<SmallTile>(ps, phase, wide, cost[2])};
+        int best = 0;
+        for (int i = 0; i < 3; ++i) {
+            l[i].tile = i;
+            if (cost[i] < cost[best]) best = i;
+        }
+        if (getenv("NS_DBG")) fprintf(stderr, "phase %d wide %d: cost %.1f (%u+%u) %.1f (%u+%u) %.1f (%u+%u)\n", phase, wide, cost[0], l[0].blocks, l[0].join_tiles, cost[1], l[1].blocks, l[1].join_tiles, cost[2], l[2].blocks, l[2].join_tiles);
+        if (const char* e = getenv(phase == GRAM ? "NS_GRAM" : phase == SQUARE ? "NS_POLY" : "NS_APPLY")) best = atoi(e);
+        return l[best];
     }
 };
 
@@ -1017,6 +1068,10 @@ struct NsLaunch {
 
 struct NewtonSchulzPlan::Group {
     NsLaunch norm, load, product[3];
+};
+struct NewtonSchulzPlan::Op {
+    int phase;
+    NsStep step;
 };
 
 NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
@@ -1027,21 +1082,98 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
     if (coef_.empty() || coef_.size() % 3)
         throw std::invalid_argument("newton_schulz: one (a, b, c) per step");
     if (!(eps >= 0) || !std::isfinite(eps)) throw std::invalid_argument("newton_schulz: bad eps");
-    // The range of the singular values after each step, from ||Y_0|| <= 1.
-    double r = 1.0, ymax = 1.0, amax = 1.0, bmax = 0.0;
-    for (size_t k = 0; k < coef_.size(); k += 3) {
-        const double a = coef_[k], b = coef_[k + 1], c = coef_[k + 2];
-        amax = std::max(amax, r * r);
-        bmax = std::max(bmax, poly2_max(b, c, r * r));
-        r = poly_max(a, b, c, r);
-        if (!(r <= 8.0) || !(bmax <= 1024.0))
-            throw std::invalid_argument("newton_schulz: step " + std::to_string(k / 3) +
+    // Ranges from ||Y_0|| <= 1 on: the singular values before each step, and the polynomial's factor.
+    const int steps = (int)coef_.size() / 3;
+    std::vector<double> sigma{1.0}, factor;
+    double ymax = 1.0;
+    for (int k = 0; k < steps; ++k) {
+        const double a = coef_[3 * k], b = coef_[3 * k + 1], c = coef_[3 * k + 2], r = sigma.back();
+        factor.push_back(factor_max(a, b, c, r * r));
+        sigma.push_back(poly_max(a, b, c, r));
+        if (!(sigma.back() <= 8.0) || !(factor.back() <= 1024.0))
+            throw std::invalid_argument("newton_schulz: step " + std::to_string(k) +
                                         " of these coefficients lets singular values grow past 8");
-        ymax = std::max(ymax, r);
+        ymax = std::max(ymax, sigma.back());
     }
     x_exp_ = scale_exp(ymax);
-    a_exp_ = scale_exp(amax);
-    b_exp_ = scale_exp(std::max(bmax, 1e-3));
+
+    // Several steps can share one A = Y Y^T and one Y <- P Y: with Q_k = a + b A_k + c A_k^2 the next
+    // step's matrix is A_(k+1) = Q_k A_k Q_k and P the product of the Q_k.  That trades 3 m^2 n
+    // multiplications per step saved for 3 m^3 (symmetric products), but the rounding of A grows by
+    // factor^2 for small singular values with every step it is carried on (simulated with the planes'
+    // roundings, three steps: 1.4 times the single steps' error at 512 rows, five: 70 times).  The
+    // products of such a chain are always wide.
+    double single = 0, shared = 0;
+    std::vector<int> groups;
+    for (int k = 0; k < steps;) {
+        int n = 1;
+        double growth = 1;
+        while (k + n < steps && n < 3) {
+            growth *= std::max(1.0, coef_[3 * (k + n - 1)] * (double)coef_[3 * (k + n - 1)]);
+            if (growth > 200) break;
+            ++n;
+        }
+        if (n == 3 && steps - k == 4) n = 2;        // 2 + 2 rather than 3 + 1
+        groups.push_back(n);
+        k += n;
+    }
+    for (const NsShape& s : shapes) {
+        const double m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols), area = m * m * s.batch;
+        single += steps * (3 * n + m) * area;
+        for (int g : groups) shared += (3 * n + (wide_ || g == 1 ? 1 : 3) * (4 * g - 3) * m) * area;
+    }
+    if (getenv("NS_SINGLE") || shared > 0.8 * single) groups.assign(steps, 1);
+    squares_wide_ = wide_ || (int)groups.size() < steps;
+    enum { A = 0, P = 1, P2 = 2, Q = 3, T = 4 };
+    int squares = 2, k = 0, buffer = 0;
+    for (int g : groups) {
+        if (g > 1) squares = kSquares;
+        double amax = sigma[k] * sigma[k], pmax = 1;
+        int ea = scale_exp(std::max(amax, 1e-3)), ep = 0, p = P;
+        NsStep s{};
+        s.sy = std::ldexp(1.f, x_exp_);
+        s.buffer = buffer;
+        auto square = [&](int x, int ex, int w, int ew, int z, int ez, float k0, float k1, float k2) {
+            NsStep t = s;
+            t.inv = std::ldexp(1.f, -ex - ew);
+            t.ix = std::ldexp(1.f, -ex);
+            t.iw = std::ldexp(1.f, -ew);
+            t.sz = std::ldexp(1.f, ez);
+            t.k0 = k0; t.k1 = k1; t.k2 = k2;
+            t.x = x; t.w = w; t.z = z;
+            ops_.push_back(std::make_shared<Op>(Op{SQUARE, t}));
+        };
+        s.inv = std::ldexp(1.f, -2 * x_exp_);
+        s.sz = std::ldexp(1.f, ea);
+        s.z = A;
+        ops_.push_back(std::make_shared<Op>(Op{GRAM, s}));
+        for (int i = 0; i < g; ++i, ++k) {
+            const int q = i ? Q : P, eq = scale_exp(factor[k]);
+            square(A, ea, A, ea, q, eq, coef_[3 * k], coef_[3 * k + 2], coef_[3 * k + 1]);
+            if (i + 1 < g) {
+                const int et = scale_exp(std::max(factor[k] * amax, 1e-3));
+                amax = sigma[k + 1] * sigma[k + 1];
+                const int en = scale_exp(std::max(amax, 1e-3));
+                square(q, eq, A, ea, T, et, 0.f, 1.f, 0.f);
+                square(q, eq, T, et, A, en, 0.f, 1.f, 0.f);
+                ea = en;
+            }
+            pmax *= factor[k];
+            if (i) {
+                const int to = p == P ? P2 : P, en = scale_exp(pmax);
+                square(Q, eq, p, ep, to, en, 0.f, 1.f, 0.f);
+                p = to;
+                ep = en;
+            } else {
+                ep = eq;
+            }
+        }
+        s.inv = std::ldexp(1.f, -x_exp_ - ep);
+        s.x = p;
+        s.last = k == steps;
+        ops_.push_back(std::make_shared<Op>(Op{APPLY, s}));
+        buffer ^= 1;
+    }
 
     size_t at = 0;
     for (const NsShape& s : shapes) {
@@ -1055,7 +1187,7 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         if (q.n > (1 << 24)) throw std::invalid_argument("newton_schulz: dimension over 2^24");
         q.mp = round_up(q.m, kPad);
         q.np = round_up(q.n, kPad);
-        q.ws_stride = (long long)((ns_matrix_bytes(q.mp, q.np) + 255) & ~(size_t)255);
+        q.ws_stride = (long long)((ns_matrix_bytes(q.mp, q.np, squares) + 255) & ~(size_t)255);
         q.ws = (long long)at;
         at += (size_t)q.ws_stride * s.batch;
         mats_.push_back(q);
@@ -1091,8 +1223,8 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         }
         g.norm = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)p.parts; });
         g.load = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)(p.mp / 64) * (p.np / 64); });
-        for (int phase : {(int)GRAM, (int)POLY, (int)APPLY}) {
-            g.product[phase] = NsLaunch::product(ps, phase, wide_);
+        for (int phase : {(int)GRAM, (int)SQUARE, (int)APPLY}) {
+            g.product[phase] = NsLaunch::product(ps, phase, phase == SQUARE ? squares_wide_ : wide_);
             slab = std::max(slab, g.product[phase].slab_bytes);
         }
     }
@@ -1122,7 +1254,7 @@ template <typename G, bool WIDE>
 void launch_phase(const NsLaunch& l, int phase, NsType type, char* ws, float* slab, const NsStep& s,
                   const NsResult& r, hipStream_t stream) {
     if (phase == GRAM) launch_product<G, WIDE, GRAM, float>(l, ws, slab, s, r, stream);
-    else if (phase == POLY) launch_product<G, WIDE, POLY, float>(l, ws, slab, s, r, stream);
+    else if (phase == SQUARE) launch_product<G, WIDE, SQUARE, float>(l, ws, slab, s, r, stream);
     else if (type == NS_BF16) launch_product<G, WIDE, APPLY, bf16_t>(l, ws, slab, s, r, stream);
     else if (type == NS_F16) launch_product<G, WIDE, APPLY, f16_t>(l, ws, slab, s, r, stream);
     else launch_product<G, WIDE, APPLY, float>(l, ws, slab, s, r, stream);
@@ -1133,27 +1265,20 @@ void launch_phase(const NsLaunch& l, int phase, NsType type, char* ws, float* sl
 template <typename Prepare>
 void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, void* out, float* p,
                              float lr, float decay, hipStream_t stream) const {
-    NsResult r{out, p, lr, decay};
-    NsStep s{};
-    s.sx = std::ldexp(1.f, x_exp_);
-    s.sa = std::ldexp(1.f, a_exp_);
-    s.sb = std::ldexp(1.f, b_exp_);
+    const NsResult r{out, p, lr, decay};
     float* slab = (float*)(ws + slab_);
     for (const auto& g : groups_) {
-        prepare(*g, (double*)(ws + partials_), s.sx);
-        const int steps = (int)coef_.size() / 3;
-        for (int k = 0; k < steps; ++k) {
-            s.a = coef_[3 * k]; s.b = coef_[3 * k + 1]; s.c = coef_[3 * k + 2];
-            s.buffer = k & 1;
-            s.last = k == steps - 1;
-            for (int phase : {(int)GRAM, (int)POLY, (int)APPLY}) {
-                s.inv = std::ldexp(1.f, phase == GRAM ? -2 * x_exp_ : phase == POLY ? -2 * a_exp_ : -x_exp_ - b_exp_);
-                const NsLaunch& l = g->product[phase];
-                if (l.big && wide_) launch_phase<BigTile, true>(l, phase, type, ws, slab, s, r, stream);
-                else if (l.big) launch_phase<BigTile, false>(l, phase, type, ws, slab, s, r, stream);
-                else if (wide_) launch_phase<SmallTile, true>(l, phase, type, ws, slab, s, r, stream);
-                else launch_phase<SmallTile, false>(l, phase, type, ws, slab, s, r, stream);
-            }
+        prepare(*g, (double*)(ws + partials_), std::ldexp(1.f, x_exp_));
+        for (const auto& op : ops_) {
+            const NsLaunch& l = g->product[op->phase];
+            auto go = [&](auto tile) {
+                typedef decltype(tile) G;
+                if (op->phase == SQUARE ? squares_wide_ : wide_) launch_phase<G, true>(l, op->phase, type, ws, slab, op->step, r, stream);
+                else launch_phase<G, false>(l, op->phase, type, ws, slab, op->step, r, stream);
+            };
+            if (l.tile == 0) go(BigTile{});
+            else if (l.tile == 1) go(MidTile{});
+            else go(SmallTile{});
         }
     }
 }
