@@ -44,9 +44,10 @@ struct MuonArgs {
 class NewtonSchulzPlan {
   public:
     // `coefficients`: one (a, b, c) per step.  `wide_products`: keep 22 bits of every factor of a
-    // matrix product (two fp16 terms, three products) instead of 11.
+    // matrix product (two fp16 terms, three products) instead of 11.  `fine_result`: the result
+    // itself is kept in fp32 (an update adds a small multiple of it to the weights).
     NewtonSchulzPlan(const std::vector<NsShape>& shapes, const std::vector<NsSegment>& segments,
-                     const std::vector<float>& coefficients, double eps, bool wide_products);
+                     const std::vector<float>& coefficients, double eps, bool wide_products, bool fine_result);
     size_t workspace_bytes() const { return ws_bytes_; }
     // out = NewtonSchulz(x); the workspace (256-byte aligned) holds no state between calls.
     void orthogonalize(const void* x, void* out, NsType type, void* ws, size_t ws_bytes,
@@ -65,9 +66,13 @@ class NewtonSchulzPlan {
     struct Group;                    // the launches of as many matrices as a launch takes
     struct Op;                       // one product of the chain
     void check_workspace(const void* ws, size_t ws_bytes) const;
-    template <typename Prepare>
-    void chain(char* ws, NsType type, const Prepare& prepare, void* out, float* p, float lr, float decay,
-               hipStream_t stream) const;
+    struct Solo;                     // one block per matrix
+    template <typename T, bool MUON>
+    void launch_solo(const Group& g, const void* x, const void* update, const void* result,
+                     hipStream_t stream) const;
+    template <typename Prepare, typename SoloRun>
+    void chain(char* ws, NsType type, const Prepare& prepare, const SoloRun& solo, void* out, float* p,
+               float lr, float decay, hipStream_t stream) const;
 
     std::vector<Matrix> mats_;
     std::vector<NsSegment> segs_;
@@ -76,6 +81,7 @@ class NewtonSchulzPlan {
     bool wide_, squares_wide_ = false;
     int x_exp_;                      // Y's planes hold value * 2^exp
     std::vector<std::shared_ptr<Op>> ops_;
+    std::shared_ptr<Solo> solo_;
     std::vector<std::shared_ptr<Group>> groups_;
     size_t partials_ = 0, slab_ = 0, ws_bytes_ = 0;      // offsets in the workspace, its size
 };

@@ -33,6 +33,7 @@ typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
 typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef const __attribute__((address_space(1))) void* global_ptr;
 typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
 typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 
 constexpr int kMaxProblems = 24;        // per launch: the table has to fit the kernel arguments
@@ -890,6 +891,251 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, con
     ns_epilogue<64, 64, LD, 256, G::kM, PHASE, OUT>(E, rows, cols, q, w, ws, b, i0, j0, s, res, put);
 }
 
+// ------------------------------------------------------------------ one block per matrix
+// Where Y and one m x m matrix fit a CU's LDS, a block runs the whole chain of a matrix by itself:
+// one launch instead of 17 or more, no memory traffic but the matrix itself.  Rows are padded to
+// multiples of 32, pitches by 8 elements so that the 16 rows of a fragment meet different banks.
+constexpr int kSoloThreads = 1024, kSoloWaves = kSoloThreads / 64;
+constexpr size_t kSoloLds = 156 * 1024;
+constexpr int kSoloParts = 16;              // partial 16 x 16 tiles of A
+constexpr int kSoloRows = 128;              // largest m: 36 tiles of A's upper triangle, 3 a wave
+
+struct SoloPlanes {                         // a matrix in LDS: hi plane, then lo plane
+    uint16_t* hi;
+    int plane, ld;
+    __device__ __forceinline__ float at(int i, int j) const {
+        return f16_value(hi[i * ld + j]) + f16_value(hi[plane + i * ld + j]);
+    }
+    __device__ __forceinline__ void put(int i, int j, float v) const {
+        uint16_t h, l;
+        split_f16(v, h, l);
+        hi[i * ld + j] = h;
+        hi[plane + i * ld + j] = l;
+    }
+    // 16 rows from i, 32 columns from k: this lane's eight
+    __device__ __forceinline__ f16x8 rows(int i, int k, int lo) const {
+        const int lane = threadIdx.x & 63;
+        return *(const f16x8*)(hi + lo * plane + (i + (lane & 15)) * ld + k + (lane >> 4) * 8);
+    }
+    // 32 rows from k, 16 columns from j, transposed
+    __device__ __forceinline__ f16x8 across(int k, int j, int lo) const {
+        const int lane = threadIdx.x & 63;
+        const uint16_t* at = hi + lo * plane + (k + (lane >> 4) * 8 + ((lane & 15) >> 2)) * ld + j + (lane & 3) * 4;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * ld));
+        const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+        return __builtin_bit_cast(f16x8, v);
+    }
+};
+__host__ __device__ inline int solo_pad(int v) { return (v + 31) / 32 * 32; }
+__host__ __device__ inline size_t solo_lds(int m, int n) {
+    const size_t mp = solo_pad(m), np = solo_pad(n);
+    return 4 * mp * (np + 8) + 4 * mp * (mp + 8) + 8 * mp + kSoloParts * 1024;
+}
+__device__ __forceinline__ f32x4 mfma_wide(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x4 acc) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, acc, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, acc, 0, 0, 0);
+}
+// Tile t of the upper triangle of 16 x 16 tiles, column by column.
+__device__ __forceinline__ void solo_tile(int t, int& ti, int& tj) {
+    tj = 0;
+    while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
+    ti = t - tj * (tj + 1) / 2;
+}
+
+struct SoloSteps {
+    int steps;
+    float sy, sa, sp;               // scales of the planes of Y, A, P
+    float k[64 * 3];                // (a, b, c) per step
+};
+
+template <typename T, bool MUON>
+__global__ __launch_bounds__(kSoloThreads) void ns_solo_kernel(NsTable tab, const T* __restrict__ x, NsUpdate u,
+                                                               double eps, SoloSteps st, NsResult res) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int problem = ns_find(tab, blockIdx.x);
+    const NsProblem& q = tab.p[problem];
+    const int b = blockIdx.x - tab.first[problem];
+    const int mp = solo_pad(q.m), np = solo_pad(q.n);
+    SoloPlanes y, sq;
+    y.hi = (uint16_t*)smem;
+    y.ld = np + 8;
+    y.plane = mp * y.ld;
+    sq.hi = y.hi + 2 * y.plane;
+    sq.ld = mp + 8;
+    sq.plane = mp * sq.ld;
+    float* d = (float*)(sq.hi + 2 * sq.plane);      // diagonal of A
+    float* e = d + mp;                              // diagonal of P
+    float* parts = e + mp;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l15 = lane & 15, lq = lane >> 4;
+
+    // norm (and momentum)
+    const long long src = q.src + b * q.stride;
+    const int count = q.rows * q.cols;
+    double sum = 0.0;
+    for (int k = tid; k < count; k += kSoloThreads) {
+        const long long at = src + (long long)(k / q.cols) * q.ld + k % q.cols;
+        float v;
+        if constexpr (MUON) {
+            const float g = u.g[at] * u.grad_scale;
+            const float m = u.mu * u.m[at] + g;
+            u.m[at] = m;
+            v = u.nesterov ? g + u.mu * m : m;
+        } else {
+            v = ns_elem(x[at]);
+        }
+        sum += (double)v * (double)v;
+    }
+    double* sums = (double*)parts;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+    if (lane == 0) sums[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+    for (int k = 0; k < kSoloWaves; ++k) sum += sums[k];
+    const double inv = (double)st.sy / (sqrt(sum) + eps);
+    for (int k = tid; k < y.plane; k += kSoloThreads) ((uint32_t*)y.hi)[k] = 0;
+    __syncthreads();
+    for (int k = tid; k < count; k += kSoloThreads) {
+        const int r = k / q.cols, c = k % q.cols;
+        const long long at = src + (long long)r * q.ld + c;
+        float v;
+        if constexpr (MUON) {
+            const float m = u.m[at];        // this thread's own, written above
+            v = u.nesterov ? u.g[at] * u.grad_scale + u.mu * m : m;
+        } else {
+            v = ns_elem(x[at]);
+        }
+        v = (float)((double)v * inv);
+        if (q.trans) y.put(c, r, v);
+        else y.put(r, c, v);
+    }
+    __syncthreads();
+
+    const int tm = mp / 16, tiles = tm * (tm + 1) / 2, ksteps = np / 32;
+    const int cuts = tiles >= kSoloParts ? 1 : (kSoloParts / tiles < ksteps ? kSoloParts / tiles : ksteps);
+    const float inv_a = 1.f / (st.sy * st.sy), inv_p = 1.f / (st.sa * st.sa), inv_y = 1.f / (st.sp * st.sy);
+    constexpr int kOwn = (kSoloRows / 16 * (kSoloRows / 16 + 1) / 2 + kSoloWaves - 1) / kSoloWaves;
+    for (int step = 0; step < st.steps; ++step) {
+        const float ka = st.k[3 * step], kb = st.k[3 * step + 1], kc = st.k[3 * step + 2];
+        f32x4 acc[kOwn];
+        // A = Y Y^T: a wave takes tiles of the upper triangle or, where they are few, parts of their sums
+        if (cuts > 1) {
+            if (wave < tiles * cuts) {
+                int ti, tj;
+                solo_tile(wave / cuts, ti, tj);
+                const int cut = wave % cuts;
+                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+                for (int k = ksteps * cut / cuts; k < ksteps * (cut + 1) / cuts; ++k)
+                    a = mfma_wide(y.rows(ti * 16, k * 32, 0), y.rows(ti * 16, k * 32, 1), y.rows(tj * 16, k * 32, 0),
+                                  y.rows(tj * 16, k * 32, 1), a);
+                *(f32x4*)(parts + (wave * 64 + lane) * 4) = a;
+            }
+            __syncthreads();
+        }
+#pragma unroll
+        for (int n = 0; n < kOwn; ++n) {
+            const int t = wave + n * kSoloWaves;
+            if (t >= tiles) break;
+            int ti, tj;
+            solo_tile(t, ti, tj);
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            if (cuts > 1) {
+                for (int k = 0; k < cuts; ++k) a += *(const f32x4*)(parts + ((t * cuts + k) * 64 + lane) * 4);
+            } else {
+                for (int k = 0; k < ksteps; ++k)
+                    a = mfma_wide(y.rows(ti * 16, k * 32, 0), y.rows(ti * 16, k * 32, 1), y.rows(tj * 16, k * 32, 0),
+                                  y.rows(tj * 16, k * 32, 1), a);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = ti * 16 + lq * 4 + r, j = tj * 16 + l15;
+                float z = a[r] * inv_a;
+                if (i == j) {
+                    d[i] = z;
+                    z = 0.f;
+                }
+                sq.put(i, j, z * st.sa);
+                if (ti != tj) sq.put(j, i, z * st.sa);
+            }
+        }
+        __syncthreads();
+        // P = b A + c A A in place of A, its diagonal with the a
+#pragma unroll
+        for (int n = 0; n < kOwn; ++n) {
+            const int t = wave + n * kSoloWaves;
+            if (t >= tiles) break;
+            int ti, tj;
+            solo_tile(t, ti, tj);
+            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < mp / 32; ++k)
+                a = mfma_wide(sq.rows(ti * 16, k * 32, 0), sq.rows(ti * 16, k * 32, 1), sq.rows(tj * 16, k * 32, 0),
+                              sq.rows(tj * 16, k * 32, 1), a);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = ti * 16 + lq * 4 + r, j = tj * 16 + l15;
+                const float di = d[i], dj = d[j], o = sq.at(i, j) / st.sa, z = a[r] * inv_p;
+                acc[n][r] = i == j ? kc * (z + di * di) + (kb * di + ka) : kc * (z + (di + dj) * o) + kb * o;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < kOwn; ++n) {
+            const int t = wave + n * kSoloWaves;
+            if (t >= tiles) break;
+            int ti, tj;
+            solo_tile(t, ti, tj);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int i = ti * 16 + lq * 4 + r, j = tj * 16 + l15;
+                float z = acc[n][r];
+                if (i == j) {
+                    e[i] = z;
+                    z = 0.f;
+                }
+                sq.put(i, j, z * st.sp);
+                if (ti != tj) sq.put(j, i, z * st.sp);
+            }
+        }
+        __syncthreads();
+        // Y <- P Y: a wave takes columns, whose old values it has read before it writes the new ones
+        const bool last = step == st.steps - 1;
+        for (int tj = wave; tj < np / 16; tj += kSoloWaves) {
+            f16x8 ch[kSoloRows / 32], cl[kSoloRows / 32];
+#pragma unroll
+            for (int k = 0; k < kSoloRows / 32; ++k)
+                if (k < mp / 32) {
+                    ch[k] = y.across(k * 32, tj * 16, 0);
+                    cl[k] = y.across(k * 32, tj * 16, 1);
+                }
+            for (int ti = 0; ti < tm; ++ti) {
+                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < kSoloRows / 32; ++k)
+                    if (k < mp / 32) a = mfma_wide(sq.rows(ti * 16, k * 32, 0), sq.rows(ti * 16, k * 32, 1), ch[k], cl[k], a);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = ti * 16 + lq * 4 + r, j = tj * 16 + l15;
+                    const float z = e[i] * (y.at(i, j) / st.sy) + a[r] * inv_y;
+                    if (!last) {
+                        y.put(i, j, z * st.sy);
+                    } else if (i < q.m && j < q.n) {
+                        const long long row = q.trans ? j : i, col = q.trans ? i : j;
+                        if (MUON) {
+                            float* at = res.p + src + row * q.ld + col;
+                            *at = res.decay * *at - res.lr * q.lr * z;
+                        } else {
+                            ((T*)res.out)[q.out + b * q.out_stride + row * q.out_ld + col] = (T)z;
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
 // Largest |a x + b x^3 + c x^5| over [0, r].
@@ -1067,7 +1313,11 @@ struct NsLaunch {
 }  // namespace
 
 struct NewtonSchulzPlan::Group {
-    NsLaunch norm, load, product[3];
+    NsLaunch norm, load, product[3], solo;
+};
+struct NewtonSchulzPlan::Solo {
+    SoloSteps steps;
+    size_t lds = 0;             // 0: the matrices do not fit
 };
 struct NewtonSchulzPlan::Op {
     int phase;
@@ -1077,7 +1327,7 @@ struct NewtonSchulzPlan::Op {
 NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
                                    const std::vector<NsSegment>& segments,
                                    const std::vector<float>& coefficients, double eps,
-                                   bool wide_products)
+                                   bool wide_products, bool fine_result)
     : segs_(segments), coef_(coefficients), eps_(eps), wide_(wide_products) {
     if (coef_.empty() || coef_.size() % 3)
         throw std::invalid_argument("newton_schulz: one (a, b, c) per step");
@@ -1123,8 +1373,35 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         for (int g : groups) shared += (3 * n + (wide_ || g == 1 ? 1 : 3) * (4 * g - 3) * m) * area;
     }
     if (getenv("NS_SINGLE") || shared > 0.8 * single) groups.assign(steps, 1);
+    // Few rows do not average that rounding out: against 64 bits an fp32 result of 32 .. 128 rows is 1.3
+    // to 6 times as far off as one of single steps in plain fp32, one of 192 rows and more 0.9 to 1.15.
+    if (fine_result)
+        for (const NsShape& s : shapes)
+            if (std::min(s.rows, s.cols) < 192) groups.assign(steps, 1);
     squares_wide_ = wide_ || (int)groups.size() < steps;
     enum { A = 0, P = 1, P2 = 2, Q = 3, T = 4 };
+    // One block per matrix where all of them fit one (next to larger ones they cost nothing extra).
+    solo_ = std::make_shared<Solo>();
+    bool all = steps <= 64;
+    size_t lds = 0;
+    double fmax = 1e-3, smax = 1e-3;
+    for (const NsShape& s : shapes) {
+        const int m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols);
+        all = all && m <= kSoloRows && n <= 4096 && solo_lds(m, n) <= kSoloLds;
+        if (all) lds = std::max(lds, solo_lds(m, n));
+    }
+    for (int i = 0; i < steps; ++i) {
+        fmax = std::max(fmax, factor[i]);
+        smax = std::max(smax, sigma[i] * sigma[i]);
+        for (int j = 0; j < 3 && i < 64; ++j) solo_->steps.k[3 * i + j] = coef_[3 * i + j];
+    }
+    if (all && !shapes.empty()) {
+        solo_->lds = lds;
+        solo_->steps.steps = steps;
+        solo_->steps.sy = std::ldexp(1.f, x_exp_);
+        solo_->steps.sa = std::ldexp(1.f, scale_exp(smax));
+        solo_->steps.sp = std::ldexp(1.f, scale_exp(fmax));
+    }
     int squares = 2, k = 0, buffer = 0;
     for (int g : groups) {
         if (g > 1) squares = kSquares;
@@ -1221,6 +1498,7 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
             if (partials > 0x7fffffffLL) throw std::invalid_argument("newton_schulz: too many matrices");
             ps.push_back(p);
         }
+        g.solo = NsLaunch::simple(ps, [](const NsProblem&) { return 1LL; });
         g.norm = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)p.parts; });
         g.load = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)(p.mp / 64) * (p.np / 64); });
         for (int phase : {(int)GRAM, (int)SQUARE, (int)APPLY}) {
@@ -1262,12 +1540,28 @@ void launch_phase(const NsLaunch& l, int phase, NsType type, char* ws, float* sl
 
 }  // namespace
 
-template <typename Prepare>
-void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, void* out, float* p,
-                             float lr, float decay, hipStream_t stream) const {
+template <typename T, bool MUON>
+void NewtonSchulzPlan::launch_solo(const Group& g, const void* x, const void* update, const void* result,
+                                   hipStream_t stream) const {
+    // (more than the default 64 KB of LDS has to be allowed once per device)
+    const void* f = (const void*)ns_solo_kernel<T, MUON>;
+    if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kSoloLds) != hipSuccess)
+        throw std::runtime_error("newton_schulz: hipFuncSetAttribute");
+    hipLaunchKernelGGL((ns_solo_kernel<T, MUON>), dim3(g.solo.blocks), dim3(kSoloThreads), solo_->lds, stream,
+                       g.solo.tab, (const T*)x, *(const NsUpdate*)update, eps_, solo_->steps,
+                       *(const NsResult*)result);
+}
+
+template <typename Prepare, typename SoloRun>
+void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, const SoloRun& solo, void* out,
+                             float* p, float lr, float decay, hipStream_t stream) const {
     const NsResult r{out, p, lr, decay};
     float* slab = (float*)(ws + slab_);
     for (const auto& g : groups_) {
+        if (solo_->lds) {
+            solo(*g, r);
+            continue;
+        }
         prepare(*g, (double*)(ws + partials_), std::ldexp(1.f, x_exp_));
         for (const auto& op : ops_) {
             const NsLaunch& l = g->product[op->phase];
@@ -1300,7 +1594,13 @@ void NewtonSchulzPlan::orthogonalize(const void* x, void* out, NsType type, void
         else if (type == NS_F16) go(f16_t{});
         else go(0.f);
     };
-    chain((char*)ws, type, prepare, out, nullptr, 0.f, 0.f, stream);
+    auto solo = [&](const Group& g, const NsResult& r) {
+        const NsUpdate none{};
+        if (type == NS_BF16) launch_solo<bf16_t, false>(g, x, &none, &r, stream);
+        else if (type == NS_F16) launch_solo<f16_t, false>(g, x, &none, &r, stream);
+        else launch_solo<float, false>(g, x, &none, &r, stream);
+    };
+    chain((char*)ws, type, prepare, solo, out, nullptr, 0.f, 0.f, stream);
 }
 
 void NewtonSchulzPlan::muon(float* p, const float* g, float* m, const MuonArgs& a, void* ws,
@@ -1330,7 +1630,8 @@ void NewtonSchulzPlan::muon(float* p, const float* g, float* m, const MuonArgs& 
         hipLaunchKernelGGL((ns_load_kernel<float, true>), dim3(gr.load.blocks), dim3(256), 0, stream,
                            gr.load.tab, (const float*)nullptr, u, partials, (char*)ws, eps_, scale);
     };
-    chain((char*)ws, NS_F32, prepare, nullptr, p, a.lr, 1.f - a.lr * a.weight_decay, stream);
+    auto solo = [&](const Group& gr, const NsResult& r) { launch_solo<float, true>(gr, nullptr, &u, &r, stream); };
+    chain((char*)ws, NS_F32, prepare, solo, nullptr, p, a.lr, 1.f - a.lr * a.weight_decay, stream);
 }
 
 }  // namespace dml
