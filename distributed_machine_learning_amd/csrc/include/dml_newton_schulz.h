@@ -58,11 +58,6 @@ class NewtonSchulzPlan {
               hipStream_t stream) const;
 
   private:
-    struct Matrix {
-        NsShape s;
-        int m, n, mp, np;
-        long long ws, ws_stride;     // workspace of the first matrix and between matrices, bytes
-    };
     struct Group;                    // the launches of as many matrices as a launch takes
     struct Op;                       // one product of the chain
     void check_workspace(const void* ws, size_t ws_bytes) const;
@@ -74,7 +69,6 @@ class NewtonSchulzPlan {
     void chain(char* ws, NsType type, const Prepare& prepare, const SoloRun& solo, void* out, float* p,
                float lr, float decay, hipStream_t stream) const;
 
-    std::vector<Matrix> mats_;
     std::vector<NsSegment> segs_;
     std::vector<float> coef_;
     double eps_;

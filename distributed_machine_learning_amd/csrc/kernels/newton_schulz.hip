@@ -17,8 +17,6 @@
 // bits on [512, 4608]: 1e-4 of the result's norm; with the diagonals left in, 3e-3).
 #include <algorithm>
 #include <cmath>
-#include <cstdio>
-#include <cstdlib>
 #include <stdexcept>
 #include <string>
 
@@ -39,6 +37,7 @@ typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
 constexpr int kMaxProblems = 24;        // per launch: the table has to fit the kernel arguments
 constexpr int kPad = 64;                // planes are zero-padded to multiples of this
 constexpr int kMaxPartials = 1024;      // blocks (partial sums of squares) per matrix
+constexpr int kMaxSteps = 64;
 constexpr int kCus = 256;
 
 // Kinds of products: A = Y Y^T; Z = X W of two m x m polynomials in one A; Y <- P Y.
@@ -330,21 +329,27 @@ __global__ __launch_bounds__(256) void ns_segments_kernel(NsSegments segs, float
     }
 }
 
-// Tile shapes of the products.  Tall: the summed index is long or the tiles are many.
-struct BigTile {        // 8 waves of 64 x 64, one block per CU, two stages in flight
+// Tile shapes of the products, and their measured times in microseconds with n blocks on a CU: a step
+// of the summed index takes step + step_more * n, what comes before and after the sum about
+// tile[phase] + tile_more[phase] * n.
+struct TileTimes {
+    double wide_step, narrow_step, step_more;
+    double tile[3], tile_more[3];       // GRAM, SQUARE, APPLY
+};
+struct BigTile {        // 8 waves of 64 x 64, two stages in flight
     static constexpr int kM = 128, kN = 256, kWavesM = 2, kWavesN = 4, kStages = 3, kBlocksPerCu = 1;
     static constexpr bool kTurns = true;
-    static constexpr double kWideStep = 1.0, kNarrowStep = 0.85, kTileUs = 13;
+    static constexpr TileTimes kTimes = {1.0, 0.85, 0.0, {15, 20, 14}, {0, 0, 0}};
 };
-struct MidTile {        // 4 waves of 64 x 64, two blocks per CU, one stage in flight
+struct MidTile {        // 4 waves of 64 x 64, one stage in flight
     static constexpr int kM = 128, kN = 128, kWavesM = 2, kWavesN = 2, kStages = 2, kBlocksPerCu = 2;
     static constexpr bool kTurns = false;
-    static constexpr double kWideStep = 1.4, kNarrowStep = 1.1, kTileUs = 8;
+    static constexpr TileTimes kTimes = {0.85, 0.7, 0.25, {8, 12, 8}, {0, 0, 0}};
 };
-struct SmallTile {      // 4 waves of 32 x 32, two blocks per CU, three stages in flight
-    static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 4, kBlocksPerCu = 2;
+struct SmallTile {      // 4 waves of 32 x 32, two stages in flight
+    static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 3, kBlocksPerCu = 3;
     static constexpr bool kTurns = false;
-    static constexpr double kWideStep = 0.5, kNarrowStep = 0.45, kTileUs = 4;
+    static constexpr TileTimes kTimes = {0.2, 0.18, 0.13, {4, 5, 3}, {1.5, 2, 1}};
 };
 
 // This wave's loads but the last N have landed and its LDS reads are done, then so for all waves.
@@ -750,22 +755,22 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
 #pragma unroll
     for (int n = 0; n < G::kStages - 1; ++n)
         if (n < steps) stage(n);
-    f16x8 fr[2][FM], fc[2][FN];
-    auto read = [&](int k) {
+    struct Fragments { f16x8 r[2][FM], c[2][FN]; };
+    auto read = [&](int k, Fragments& f) {
         const char* sr = smem + (k % G::kStages) * kStage;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int x = 0; x < FM; ++x) {
                 const int r = wi + x * 16 + l15;
-                fr[h][x] = *(const f16x8*)(sr + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
+                f.r[h][x] = *(const f16x8*)(sr + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
             }
         if constexpr (PHASE == APPLY) {
             unsigned at[FN];
 #pragma unroll
             for (int y = 0; y < FN; ++y) at[y] = across[y] + (unsigned)(k % G::kStages) * kStage;
-            read_across<FN, 0, 4 * G::kN * 2>(at, fc[0]);
-            read_across<FN, 32 * G::kN * 2, 4 * G::kN * 2>(at, fc[1]);
+            read_across<FN, 0, 4 * G::kN * 2>(at, f.c[0]);
+            read_across<FN, 32 * G::kN * 2, 4 * G::kN * 2>(at, f.c[1]);
         } else {
             const char* sc = sr + G::kM * 128;
 #pragma unroll
@@ -773,11 +778,11 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
 #pragma unroll
                 for (int y = 0; y < FN; ++y) {
                     const int r = wj + y * 16 + l15;
-                    fc[h][y] = *(const f16x8*)(sc + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
+                    f.c[h][y] = *(const f16x8*)(sc + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
                 }
         }
     };
-    auto multiply = [&]() {
+    auto multiply = [&](const Fragments& f) {
 #pragma unroll
         for (int n = 0; n < (WIDE ? 3 : 2); ++n)        // hi hi, hi lo, lo hi; or two halves of the step
 #pragma unroll
@@ -785,7 +790,7 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
 #pragma unroll
                 for (int y = 0; y < FN; ++y)
                     acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        fc[WIDE ? n >> 1 : n][y], fr[WIDE ? n & 1 : n][x], acc[x][y], 0, 0, 0);
+                        f.c[WIDE ? n >> 1 : n][y], f.r[WIDE ? n & 1 : n][x], acc[x][y], 0, 0, 0);
     };
     auto await = [&](int k) {
         if (k + G::kStages - 2 < steps) await_stage<(G::kStages - 2) * kLoads>();
@@ -796,24 +801,45 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
         // products of the other one run, and neither the LDS nor the matrix unit waits for the
         // other.  The second half of the waves is one barrier behind; a stage has landed before the
         // first half reads it and is refilled after the second half has.
+        Fragments f;
         const bool second = __builtin_amdgcn_readfirstlane(wave) >= kWaves / 2;
         if (second) await(0);
         for (int k = 0; k < steps; ++k) {
             if (second) turn();
             else await(k);
-            read(k);
+            read(k, f);
             if (k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
             if (second) await(k + 1);
             else turn();
-            multiply();
+            multiply(f);
         }
         if (!second) turn();
+    } else if constexpr (PHASE != APPLY) {
+        // A wave reads the fragments of a step while the products of the step before run.  All waves
+        // have read stage k when they pass the barrier of step k, so it is refilled at once.
+        Fragments f0, f1;
+        if (G::kStages - 1 < steps) stage(G::kStages - 1);
+        await(0);
+        read(0, f0);
+        auto step = [&](int k, const Fragments& now, Fragments& next) {
+            if (k + 1 < steps) {
+                await(k + 1);
+                if (k + G::kStages < steps) stage(k + G::kStages);
+                read(k + 1, next);
+            }
+            multiply(now);
+        };
+        for (int k = 0; k < steps; k += 2) {
+            step(k, f0, f1);
+            if (k + 1 < steps) step(k + 1, f1, f0);
+        }
     } else {
+        Fragments f;
         for (int k = 0; k < steps; ++k) {
             await(k);
             if (k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
-            read(k);
-            multiply();
+            read(k, f);
+            multiply(f);
         }
     }
     if (it.split >= 0) {        // fragments of 16 x 16, lane by lane
@@ -896,6 +922,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, con
 // one launch instead of 17 or more, no memory traffic but the matrix itself.  Rows are padded to
 // multiples of 32, pitches by 8 elements so that the 16 rows of a fragment meet different banks.
 constexpr int kSoloThreads = 1024, kSoloWaves = kSoloThreads / 64;
+constexpr int kSoloCols = 4096;
 constexpr size_t kSoloLds = 156 * 1024;
 constexpr int kSoloParts = 16;              // partial 16 x 16 tiles of A
 constexpr int kSoloRows = 128;              // largest m: 36 tiles of A's upper triangle, 3 a wave
@@ -947,8 +974,9 @@ __device__ __forceinline__ void solo_tile(int t, int& ti, int& tj) {
 struct SoloSteps {
     int steps;
     float sy, sa, sp;               // scales of the planes of Y, A, P
-    float k[64 * 3];                // (a, b, c) per step
+    float k[3 * kMaxSteps];         // (a, b, c) per step
 };
+static_assert(sizeof(NsTable) + sizeof(SoloSteps) <= 4000, "kernel arguments");
 
 template <typename T, bool MUON>
 __global__ __launch_bounds__(kSoloThreads) void ns_solo_kernel(NsTable tab, const T* __restrict__ x, NsUpdate u,
@@ -1176,6 +1204,7 @@ struct NsLaunch {
     NsTable tab, join;          // `join`: the split entries, counted in tiles
     unsigned blocks = 0, join_tiles = 0;
     int tile = 0;               // 0 big, 1 mid, 2 small
+    double cost = 0;            // estimate, us
     size_t slab_bytes = 0;
 
     static int checked(long long blocks) {
@@ -1205,12 +1234,11 @@ struct NsLaunch {
     }
     // Tiles fill the chip a round of kCus * kBlocksPerCu at a time.  Where they fill less than three
     // quarters of the last round, its tiles' summed index may be divided until they do; whether it is
-    // goes by the estimate `cost` in microseconds (the tile shapes' measured constants).
+    // goes by the estimate in microseconds that is left in `cost`.
     template <typename G>
     static NsLaunch tiled(const std::vector<NsProblem>& ps, int phase, bool wide, double& cost) {
         constexpr int kSlots = kCus * G::kBlocksPerCu;
         constexpr int kShortest = 4;            // steps of the shortest part
-        const double step_us = wide ? G::kWideStep : G::kNarrowStep;
         const int step = wide ? 32 : 64;
         NsLaunch l{};
         struct Entry { NsProblem p; long long begin, count; int splits; };
@@ -1222,10 +1250,19 @@ struct NsLaunch {
             total += checked(tiles_of<G>(p, phase)) * (long long)p.batch;
             longest = std::max(longest, steps_of(p));
         }
-        auto join_us = [&](long long items) { return 7.0 + (double)items * G::kM * G::kN * 8 / 4e6; };
-        const long long rest = total % kSlots, rounds = (total + kSlots - 1) / kSlots;
+        // one round of `blocks` with sums of `steps`, `finish`: the share of the tile's own time
+        auto round_us = [&](long long blocks, double steps, double finish) {
+            const TileTimes& t = G::kTimes;
+            const double n = (double)std::min<long long>(G::kBlocksPerCu, (blocks + kCus - 1) / kCus);
+            return steps * ((wide ? t.wide_step : t.narrow_step) + t.step_more * n) +
+                   finish * (t.tile[phase] + t.tile_more[phase] * n);
+        };
+        // the joining launch: its latency, and the parts written and read at 4 TB/s
+        auto join_us = [&](long long items) { return 9.0 + (double)items * G::kM * G::kN * 8 / 4e6; };
+        const long long rest = total % kSlots;
+        const double full = (total / kSlots) * round_us(kSlots, longest, 1);
         long long keep = total;         // tiles that stay whole
-        cost = rounds * (longest * step_us + G::kTileUs);
+        cost = full + (rest ? round_us(rest, longest, 1) : 0);
         if (rest && rest * 4 <= kSlots * 3) {
             if (total < kSlots) {       // one round: parts of equal length, of all that are longer
                 int part = longest;
@@ -1236,7 +1273,7 @@ struct NsLaunch {
                         items += tiles_of<G>(p, phase) * p.batch * ((steps_of(p) + n - 1) / n);
                     if (items <= kSlots) { part = n; break; }
                 }
-                const double divided = part * step_us + 0.5 * G::kTileUs + join_us(items);
+                const double divided = round_us(items, part, 0.5) + join_us(items);
                 if (part < longest && divided < cost) {
                     cost = divided;
                     keep = 0;
@@ -1249,8 +1286,7 @@ struct NsLaunch {
             } else {
                 const int parts = (int)std::min<long long>(kSlots / rest, steps_of(ps.back()) / kShortest);
                 if (parts > 1) {
-                    const double divided = (rounds - 1) * (longest * step_us + G::kTileUs) +
-                                           (double)longest / parts * step_us + 0.5 * G::kTileUs + join_us(rest * parts);
+                    const double divided = full + round_us(rest * parts, (double)longest / parts, 0.5) + join_us(rest * parts);
                     if (divided < cost) {
                         cost = divided;
                         keep = total - rest;
@@ -1304,8 +1340,7 @@ struct NsLaunch {
             l[i].tile = i;
             if (cost[i] < cost[best]) best = i;
         }
-        if (getenv("NS_DBG")) fprintf(stderr, "phase %d wide %d: cost %.1f (%u+%u) %.1f (%u+%u) %.1f (%u+%u)\n", phase, wide, cost[0], l[0].blocks, l[0].join_tiles, cost[1], l[1].blocks, l[1].join_tiles, cost[2], l[2].blocks, l[2].join_tiles);
-        if (const char* e = getenv(phase == GRAM ? "NS_GRAM" : phase == SQUARE ? "NS_POLY" : "NS_APPLY")) best = atoi(e);
+        l[best].cost = cost[best] + 2.5 + (l[best].join_tiles ? 1.0 : 0.0);
         return l[best];
     }
 };
@@ -1313,11 +1348,21 @@ struct NsLaunch {
 }  // namespace
 
 struct NewtonSchulzPlan::Group {
-    NsLaunch norm, load, product[3], solo;
+    NsLaunch norm, load, product[3], wide_square, solo;
+    // The workspace of the problem whose partial sums start at `part`, in every table.
+    void place(int part, long long ws, long long stride) {
+        for (NsTable* t : {&norm.tab, &load.tab, &product[0].tab, &product[1].tab, &product[2].tab,
+                           &product[0].join, &product[1].join, &product[2].join})
+            for (int i = 0; i < t->count; ++i)
+                if (t->p[i].part == part) {
+                    t->p[i].ws = ws;
+                    t->p[i].ws_stride = stride;
+                }
+    }
 };
 struct NewtonSchulzPlan::Solo {
-    SoloSteps steps;
-    size_t lds = 0;             // 0: the matrices do not fit
+    SoloSteps steps{};
+    size_t lds = 0;
 };
 struct NewtonSchulzPlan::Op {
     int phase;
@@ -1329,13 +1374,12 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
                                    const std::vector<float>& coefficients, double eps,
                                    bool wide_products, bool fine_result)
     : segs_(segments), coef_(coefficients), eps_(eps), wide_(wide_products) {
-    if (coef_.empty() || coef_.size() % 3)
-        throw std::invalid_argument("newton_schulz: one (a, b, c) per step");
+    if (coef_.empty() || coef_.size() % 3 || coef_.size() > 3 * kMaxSteps)
+        throw std::invalid_argument("newton_schulz: one (a, b, c) per step, at most 64");
     if (!(eps >= 0) || !std::isfinite(eps)) throw std::invalid_argument("newton_schulz: bad eps");
     // Ranges from ||Y_0|| <= 1 on: the singular values before each step, and the polynomial's factor.
     const int steps = (int)coef_.size() / 3;
     std::vector<double> sigma{1.0}, factor;
-    double ymax = 1.0;
     for (int k = 0; k < steps; ++k) {
         const double a = coef_[3 * k], b = coef_[3 * k + 1], c = coef_[3 * k + 2], r = sigma.back();
         factor.push_back(factor_max(a, b, c, r * r));
@@ -1343,68 +1387,116 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         if (!(sigma.back() <= 8.0) || !(factor.back() <= 1024.0))
             throw std::invalid_argument("newton_schulz: step " + std::to_string(k) +
                                         " of these coefficients lets singular values grow past 8");
-        ymax = std::max(ymax, sigma.back());
     }
-    x_exp_ = scale_exp(ymax);
+    x_exp_ = scale_exp(*std::max_element(sigma.begin(), sigma.end()));
+
+    // Problems by falling length of their sums: a launch's last blocks are then its cheapest.
+    std::vector<NsShape> order = shapes;
+    int smallest = 1 << 30;
+    for (const NsShape& s : shapes) {
+        if (s.rows <= 0 || s.cols <= 0 || s.batch <= 0 || s.ld < s.cols || s.offset < 0 || s.stride < 0 ||
+            s.out_offset < 0)
+            throw std::invalid_argument("newton_schulz: bad matrix");
+        if (std::max(s.rows, s.cols) > (1 << 24)) throw std::invalid_argument("newton_schulz: dimension over 2^24");
+        smallest = std::min({smallest, s.rows, s.cols});
+    }
+    std::stable_sort(order.begin(), order.end(), [](const NsShape& x, const NsShape& y) {
+        return std::max(x.rows, x.cols) > std::max(y.rows, y.cols);
+    });
+    std::vector<std::vector<NsProblem>> sets;
+    long long partials = 0;
+    bool solo = !shapes.empty();
+    size_t lds = 0;
+    for (const NsShape& s : order) {
+        // (a set may need one entry more than it has problems: see NsLaunch::tiled)
+        if (sets.empty() || sets.back().size() == kMaxProblems - 1) sets.emplace_back();
+        NsProblem p{};
+        p.rows = s.rows; p.cols = s.cols; p.batch = s.batch;
+        p.m = std::min(s.rows, s.cols);
+        p.n = std::max(s.rows, s.cols);
+        p.mp = round_up(p.m, kPad);
+        p.np = round_up(p.n, kPad);
+        p.trans = s.rows > s.cols;
+        p.src = s.offset; p.ld = s.ld; p.stride = s.stride;
+        p.out = s.out_offset; p.out_ld = s.out_ld; p.out_stride = s.out_stride;
+        p.lr = s.lr;
+        p.splits = 1;
+        const bool flat = p.ld == p.cols;
+        const long long cols = flat ? (long long)p.rows * p.cols : p.cols;
+        const long long units = (cols + 2047) / 2048 * (flat ? 1 : p.rows);
+        p.parts = (int)std::min<long long>((units + 3) / 4, kMaxPartials);
+        p.part = (int)partials;
+        partials += (long long)p.batch * p.parts;
+        if (partials > 0x7fffffffLL) throw std::invalid_argument("newton_schulz: too many matrices");
+        sets.back().push_back(p);
+        solo = solo && p.m <= kSoloRows && p.n <= kSoloCols && solo_lds(p.m, p.n) <= kSoloLds;
+        if (solo) lds = std::max(lds, solo_lds(p.m, p.n));
+    }
+
+    // One block per matrix where all of them fit one (next to larger ones they cost nothing extra).
+    if (solo) {
+        solo_ = std::make_shared<Solo>();
+        solo_->lds = lds;
+        SoloSteps& st = solo_->steps;
+        st.steps = steps;
+        double amax = 1e-3;
+        for (int k = 0; k < steps; ++k) amax = std::max(amax, sigma[k] * sigma[k]);
+        st.sy = std::ldexp(1.f, x_exp_);
+        st.sa = std::ldexp(1.f, scale_exp(amax));
+        st.sp = std::ldexp(1.f, scale_exp(*std::max_element(factor.begin(), factor.end())));
+        std::copy(coef_.begin(), coef_.end(), st.k);
+        for (const auto& ps : sets) {
+            groups_.push_back(std::make_shared<Group>());
+            groups_.back()->solo = NsLaunch::simple(ps, [](const NsProblem&) { return 1LL; });
+        }
+        return;
+    }
 
     // Several steps can share one A = Y Y^T and one Y <- P Y: with Q_k = a + b A_k + c A_k^2 the next
     // step's matrix is A_(k+1) = Q_k A_k Q_k and P the product of the Q_k.  That trades 3 m^2 n
-    // multiplications per step saved for 3 m^3 (symmetric products), but the rounding of A grows by
-    // factor^2 for small singular values with every step it is carried on (simulated with the planes'
-    // roundings, three steps: 1.4 times the single steps' error at 512 rows, five: 70 times).  The
-    // products of such a chain are always wide.
-    double single = 0, shared = 0;
-    std::vector<int> groups;
+    // multiplications per step saved for 3 m^3 (symmetric products, always wide), and the rounding of A
+    // grows by a^2 for small singular values with every step that A is carried on: three steps have
+    // 1.4 times the single steps' error at 512 rows, five 70 times (simulated with the planes'
+    // roundings).  Few rows do not average it out: against 64 bits an fp32 result of 32 .. 128 rows is
+    // 1.3 to 6 times as far off as plain fp32 products, one of 192 rows and more 0.9 to 1.15 times.
+    std::vector<int> chains;
     for (int k = 0; k < steps;) {
         int n = 1;
         double growth = 1;
-        while (k + n < steps && n < 3) {
-            growth *= std::max(1.0, coef_[3 * (k + n - 1)] * (double)coef_[3 * (k + n - 1)]);
+        while (k + n < steps && n < 3 && !(fine_result && smallest < 192)) {
+            const double a = coef_[3 * (k + n - 1)];
+            growth *= std::max(1.0, a * a);
             if (growth > 200) break;
             ++n;
         }
         if (n == 3 && steps - k == 4) n = 2;        // 2 + 2 rather than 3 + 1
-        groups.push_back(n);
+        chains.push_back(n);
         k += n;
     }
-    for (const NsShape& s : shapes) {
-        const double m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols), area = m * m * s.batch;
-        single += steps * (3 * n + m) * area;
-        for (int g : groups) shared += (3 * n + (wide_ || g == 1 ? 1 : 3) * (4 * g - 3) * m) * area;
+    double single_us = 0, chain_us = 0;
+    for (const auto& ps : sets) {
+        groups_.push_back(std::make_shared<Group>());
+        Group& g = *groups_.back();
+        g.norm = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)p.parts; });
+        g.load = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)(p.mp / 64) * (p.np / 64); });
+        for (int phase : {(int)GRAM, (int)SQUARE, (int)APPLY}) g.product[phase] = NsLaunch::product(ps, phase, wide_);
+        g.wide_square = NsLaunch::product(ps, SQUARE, true);
+        const double ends = g.product[GRAM].cost + g.product[APPLY].cost;
+        single_us += steps * (ends + g.product[SQUARE].cost);
+        for (int n : chains) chain_us += ends + (4 * n - 3) * g.wide_square.cost;
     }
-    if (getenv("NS_SINGLE") || shared > 0.8 * single) groups.assign(steps, 1);
-    // Few rows do not average that rounding out: against 64 bits an fp32 result of 32 .. 128 rows is 1.3
-    // to 6 times as far off as one of single steps in plain fp32, one of 192 rows and more 0.9 to 1.15.
-    if (fine_result)
-        for (const NsShape& s : shapes)
-            if (std::min(s.rows, s.cols) < 192) groups.assign(steps, 1);
-    squares_wide_ = wide_ || (int)groups.size() < steps;
+    const bool chained = (int)chains.size() < steps && chain_us < 0.95 * single_us;
+    if (!chained) chains.assign(steps, 1);
+    size_t slab = 0;
+    for (const auto& g : groups_) {
+        if (chained) g->product[SQUARE] = g->wide_square;
+        for (const NsLaunch& l : g->product) slab = std::max(slab, l.slab_bytes);
+    }
+    squares_wide_ = wide_ || chained;
+
     enum { A = 0, P = 1, P2 = 2, Q = 3, T = 4 };
-    // One block per matrix where all of them fit one (next to larger ones they cost nothing extra).
-    solo_ = std::make_shared<Solo>();
-    bool all = steps <= 64;
-    size_t lds = 0;
-    double fmax = 1e-3, smax = 1e-3;
-    for (const NsShape& s : shapes) {
-        const int m = std::min(s.rows, s.cols), n = std::max(s.rows, s.cols);
-        all = all && m <= kSoloRows && n <= 4096 && solo_lds(m, n) <= kSoloLds;
-        if (all) lds = std::max(lds, solo_lds(m, n));
-    }
-    for (int i = 0; i < steps; ++i) {
-        fmax = std::max(fmax, factor[i]);
-        smax = std::max(smax, sigma[i] * sigma[i]);
-        for (int j = 0; j < 3 && i < 64; ++j) solo_->steps.k[3 * i + j] = coef_[3 * i + j];
-    }
-    if (all && !shapes.empty()) {
-        solo_->lds = lds;
-        solo_->steps.steps = steps;
-        solo_->steps.sy = std::ldexp(1.f, x_exp_);
-        solo_->steps.sa = std::ldexp(1.f, scale_exp(smax));
-        solo_->steps.sp = std::ldexp(1.f, scale_exp(fmax));
-    }
-    int squares = 2, k = 0, buffer = 0;
-    for (int g : groups) {
-        if (g > 1) squares = kSquares;
+    int k = 0, buffer = 0;
+    for (int n : chains) {
         double amax = sigma[k] * sigma[k], pmax = 1;
         int ea = scale_exp(std::max(amax, 1e-3)), ep = 0, p = P;
         NsStep s{};
@@ -1424,10 +1516,10 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         s.sz = std::ldexp(1.f, ea);
         s.z = A;
         ops_.push_back(std::make_shared<Op>(Op{GRAM, s}));
-        for (int i = 0; i < g; ++i, ++k) {
+        for (int i = 0; i < n; ++i, ++k) {
             const int q = i ? Q : P, eq = scale_exp(factor[k]);
             square(A, ea, A, ea, q, eq, coef_[3 * k], coef_[3 * k + 2], coef_[3 * k + 1]);
-            if (i + 1 < g) {
+            if (i + 1 < n) {
                 const int et = scale_exp(std::max(factor[k] * amax, 1e-3));
                 amax = sigma[k + 1] * sigma[k + 1];
                 const int en = scale_exp(std::max(amax, 1e-3));
@@ -1452,60 +1544,15 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         buffer ^= 1;
     }
 
+    // workspace: the matrices' planes, the partial sums, the parts of divided tiles
     size_t at = 0;
-    for (const NsShape& s : shapes) {
-        if (s.rows <= 0 || s.cols <= 0 || s.batch <= 0 || s.ld < s.cols || s.offset < 0 || s.stride < 0 ||
-            s.out_offset < 0)
-            throw std::invalid_argument("newton_schulz: bad matrix");
-        Matrix q;
-        q.s = s;
-        q.m = std::min(s.rows, s.cols);
-        q.n = std::max(s.rows, s.cols);
-        if (q.n > (1 << 24)) throw std::invalid_argument("newton_schulz: dimension over 2^24");
-        q.mp = round_up(q.m, kPad);
-        q.np = round_up(q.n, kPad);
-        q.ws_stride = (long long)((ns_matrix_bytes(q.mp, q.np, squares) + 255) & ~(size_t)255);
-        q.ws = (long long)at;
-        at += (size_t)q.ws_stride * s.batch;
-        mats_.push_back(q);
-    }
-    // long sums first: a launch's last blocks are then its cheapest
-    std::vector<Matrix> order = mats_;
-    std::stable_sort(order.begin(), order.end(), [](const Matrix& x, const Matrix& y) { return x.np > y.np; });
-    long long partials = 0;
-    size_t slab = 0;
-    for (size_t lo = 0; lo < order.size(); lo += kMaxProblems - 1) {
-        groups_.push_back(std::make_shared<Group>());
-        Group& g = *groups_.back();
-        std::vector<NsProblem> ps;
-        for (size_t i = lo; i < std::min(lo + kMaxProblems - 1, order.size()); ++i) {
-            const Matrix& q = order[i];
-            NsProblem p{};
-            p.rows = q.s.rows; p.cols = q.s.cols; p.m = q.m; p.n = q.n; p.mp = q.mp; p.np = q.np;
-            p.batch = q.s.batch;
-            p.trans = q.s.rows > q.s.cols;
-            p.src = q.s.offset; p.ld = q.s.ld; p.stride = q.s.stride;
-            p.out = q.s.out_offset; p.out_ld = q.s.out_ld; p.out_stride = q.s.out_stride;
-            p.ws = q.ws; p.ws_stride = q.ws_stride;
-            p.lr = q.s.lr;
-            p.splits = 1;
-            const bool flat = p.ld == p.cols;
-            const long long cols = flat ? (long long)p.rows * p.cols : p.cols;
-            const long long units = (cols + 2047) / 2048 * (flat ? 1 : p.rows);
-            p.parts = (int)std::min<long long>((units + 3) / 4, kMaxPartials);
-            p.part = (int)partials;
-            partials += (long long)p.batch * p.parts;
-            if (partials > 0x7fffffffLL) throw std::invalid_argument("newton_schulz: too many matrices");
-            ps.push_back(p);
+    for (size_t i = 0; i < sets.size(); ++i)
+        for (size_t j = 0; j < sets[i].size(); ++j) {
+            const NsProblem& p = sets[i][j];
+            const size_t each = (ns_matrix_bytes(p.mp, p.np, chained ? kSquares : 2) + 255) & ~(size_t)255;
+            groups_[i]->place(p.part, (long long)at, (long long)each);
+            at += each * p.batch;
         }
-        g.solo = NsLaunch::simple(ps, [](const NsProblem&) { return 1LL; });
-        g.norm = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)p.parts; });
-        g.load = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)(p.mp / 64) * (p.np / 64); });
-        for (int phase : {(int)GRAM, (int)SQUARE, (int)APPLY}) {
-            g.product[phase] = NsLaunch::product(ps, phase, phase == SQUARE ? squares_wide_ : wide_);
-            slab = std::max(slab, g.product[phase].slab_bytes);
-        }
-    }
     partials_ = at;
     at += ((size_t)partials * sizeof(double) + 255) & ~(size_t)255;
     slab_ = at;
@@ -1558,7 +1605,7 @@ void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, cons
     const NsResult r{out, p, lr, decay};
     float* slab = (float*)(ws + slab_);
     for (const auto& g : groups_) {
-        if (solo_->lds) {
+        if (solo_) {
             solo(*g, r);
             continue;
         }
@@ -1579,7 +1626,7 @@ void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, cons
 
 void NewtonSchulzPlan::orthogonalize(const void* x, void* out, NsType type, void* ws, size_t ws_bytes,
                                      hipStream_t stream) const {
-    if (mats_.empty()) return;
+    if (groups_.empty()) return;
     check_workspace(ws, ws_bytes);
     if (!x || !out) throw std::invalid_argument("newton_schulz: null matrix");
     auto prepare = [&](const Group& g, double* partials, float scale) {
@@ -1622,7 +1669,7 @@ void NewtonSchulzPlan::muon(float* p, const float* g, float* m, const MuonArgs& 
         hipLaunchKernelGGL(ns_segments_kernel, dim3(bx, (unsigned)segs.count), dim3(256), 0, stream, segs,
                            p, g, m, a.sgd_lr, a.sgd_momentum, a.sgd_weight_decay, a.grad_scale);
     }
-    if (mats_.empty()) return;
+    if (groups_.empty()) return;
     NsUpdate u{g, m, a.momentum, a.grad_scale, a.nesterov ? 1 : 0};
     auto prepare = [&](const Group& gr, double* partials, float scale) {
         hipLaunchKernelGGL((ns_norm_kernel<float, true>), dim3(gr.norm.blocks), dim3(256), 0, stream,
