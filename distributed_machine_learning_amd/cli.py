@@ -16,7 +16,7 @@ from typing import Optional, Sequence
 
 import torch
 
-from .config import SYNC_MODES, SYNC_NONE, TrainConfig, part_defaults
+from .config import OPT_MUON, OPTIMIZERS, SYNC_MODES, SYNC_NONE, TrainConfig, part_defaults
 
 
 def build_parser(defaults: TrainConfig, distributed_flags: bool = True) -> argparse.ArgumentParser:
@@ -44,6 +44,14 @@ def build_parser(defaults: TrainConfig, distributed_flags: bool = True) -> argpa
     p.add_argument("--lr", type=float, default=defaults.lr)
     p.add_argument("--momentum", type=float, default=defaults.momentum)
     p.add_argument("--weight-decay", type=float, default=defaults.weight_decay)
+    p.add_argument("--optimizer", choices=OPTIMIZERS, default=defaults.optimizer,
+                   help="muon: orthogonalised momentum for the convolution weights (--muon-*), SGD "
+                        "(--lr, --momentum, --weight-decay) for everything else")
+    p.add_argument("--muon-lr", type=float, default=defaults.muon_lr)
+    p.add_argument("--muon-momentum", type=float, default=defaults.muon_momentum)
+    p.add_argument("--muon-weight-decay", type=float, default=defaults.muon_weight_decay)
+    p.add_argument("--muon-precision", choices=("fp32", "fp16"), default=defaults.muon_precision,
+                   help="precision of the factors of Muon's matrix products")
     syn = p.add_mutually_exclusive_group()
     syn.add_argument("--synthetic", dest="synthetic", action="store_true",
                      default=defaults.synthetic)
@@ -157,6 +165,9 @@ def fun_main(cfg: TrainConfig):
     trainer = Trainer(cfg, device, comm)
     # which engine and which precision actually run (the reference is fp32 on the CPU)
     print(f"Engine: backend={trainer.backend.name}, dtype={trainer.cfg.dtype}, device={device}")
+    if cfg.optimizer == OPT_MUON:
+        print(f"Optimizer: muon, lr={cfg.muon_lr}, momentum={cfg.muon_momentum}, "
+              f"weight_decay={cfg.muon_weight_decay}, precision={cfg.muon_precision}")
     try:
         result = trainer.run()
     finally:

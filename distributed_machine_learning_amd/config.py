@@ -20,6 +20,11 @@ SYNC_ALL_REDUCE = "all_reduce"
 SYNC_DDP = "ddp"
 SYNC_MODES = (SYNC_NONE, SYNC_GATHER_SCATTER, SYNC_ALL_REDUCE, SYNC_DDP)
 
+# optimizers (the reference's is SGD)
+OPT_SGD = "sgd"
+OPT_MUON = "muon"
+OPTIMIZERS = (OPT_SGD, OPT_MUON)
+
 # CIFAR-10 channel statistics used by every variant (part1/main.py:82-83)
 CIFAR_MEAN = tuple(v / 255.0 for v in (125.3, 123.0, 113.9))
 CIFAR_STD = tuple(v / 255.0 for v in (63.0, 62.1, 66.7))
@@ -54,6 +59,13 @@ class TrainConfig:
     lr: float = 0.1
     momentum: float = 0.9
     weight_decay: float = 1e-4
+    # "muon": convolution weights take orthogonalised momentum (optim/muon.py) with the muon_*
+    # values, everything else SGD with the three values above
+    optimizer: str = OPT_SGD
+    muon_lr: float = 0.02
+    muon_momentum: float = 0.95
+    muon_weight_decay: float = 0.0
+    muon_precision: str = "fp32"           # factors of the Newton-Schulz products: "fp32" | "fp16"
     iters: int = 40                        # part1/main.py:32
     epochs: int = 1
     seed: int = SEED

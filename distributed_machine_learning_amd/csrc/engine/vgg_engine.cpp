@@ -961,10 +961,8 @@ void VggEngine::optimizer_step(float lr, float momentum, float weight_decay, flo
     repack_all(stream, bsrc, bdst, bn);
 }
 
-void VggEngine::train_step(const uint16_t* x, const int64_t* target, int batch, float lr,
-                           float momentum, float weight_decay, float grad_scale,
-                           hipStream_t stream) {
-    TraceRange range("train_step");
+void VggEngine::synced_gradients(const uint16_t* x, const int64_t* target, int batch,
+                                 hipStream_t stream) {
     forward_backward(x, target, batch, stream);
     if (manual_sync_) {
         // the two hand-written modes synchronise between backward and the update
@@ -973,7 +971,32 @@ void VggEngine::train_step(const uint16_t* x, const int64_t* target, int batch, 
                                                                         : "sync/gather_scatter");
         manual_sync_->run(stream);
     }
+}
+
+void VggEngine::train_step(const uint16_t* x, const int64_t* target, int batch, float lr,
+                           float momentum, float weight_decay, float grad_scale,
+                           hipStream_t stream) {
+    TraceRange range("train_step");
+    synced_gradients(x, target, batch, stream);
     optimizer_step(lr, momentum, weight_decay, grad_scale, stream);
+}
+
+void VggEngine::gradients_step(const uint16_t* x, const int64_t* target, int batch,
+                               hipStream_t stream) {
+    TraceRange range("train_step");
+    if (opt_.on || (reducer_ && reducer_->keeps_on_wire()))
+        throw std::logic_error("VggEngine: gradients_step() needs the fused optimizer off and the "
+                               "reduced gradients in the bound buffer");
+    synced_gradients(x, target, batch, stream);
+    if (reducer_) reducer_->wait_all(stream);
+}
+
+void VggEngine::parameters_updated(hipStream_t stream) {
+    join_update(stream);
+    const float* bsrc = nullptr; float* bdst = nullptr; size_t bn = 0;
+    if (reducer_) (void)reducer_->take_pending_buffers(&bsrc, &bdst, &bn);
+    cast_f32_to_bf16(params_, arena_ + shadow_off_, param_elems_, stream);
+    repack_all(stream, bsrc, bdst, bn);
 }
 
 void VggEngine::eval_step(const uint16_t* x, const int64_t* target, int batch, hipStream_t stream) {
@@ -1077,6 +1100,10 @@ void bind_engine(py::module_& m) {
         })
         .def("set_manual_sync", [](VggEngine& e, ManualSync* m) { e.set_manual_sync(m); },
              py::keep_alive<1, 2>())
+        .def("gradients_step", [](VggEngine& e, uintptr_t x, uintptr_t t, int batch, uintptr_t s) {
+            e.gradients_step((const uint16_t*)x, (const int64_t*)t, batch, (hipStream_t)s);
+        })
+        .def("parameters_updated", [](VggEngine& e, uintptr_t s) { e.parameters_updated((hipStream_t)s); })
         .def("optimizer_step", [](VggEngine& e, float lr, float mu, float wd, float gs, uintptr_t s) {
             e.optimizer_step(lr, mu, wd, gs, (hipStream_t)s);
         })

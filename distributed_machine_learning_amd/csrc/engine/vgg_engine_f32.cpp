@@ -502,17 +502,37 @@ void VggEngineF32::optimizer_step(float lr, float momentum, float weight_decay, 
     }
 }
 
-void VggEngineF32::train_step(const float* x, const int64_t* target, int batch, float lr,
-                              float momentum, float weight_decay, float grad_scale,
-                              hipStream_t stream) {
-    TraceRange range("train_step");
+void VggEngineF32::synced_gradients(const float* x, const int64_t* target, int batch,
+                                    hipStream_t stream) {
     forward_backward(x, target, batch, stream);
     if (manual_sync_) {
         TraceRange sync(manual_sync_->mode() == ManualSync::ALL_REDUCE ? "sync/all_reduce"
                                                                         : "sync/gather_scatter");
         manual_sync_->run(stream);
     }
+}
+
+void VggEngineF32::train_step(const float* x, const int64_t* target, int batch, float lr,
+                              float momentum, float weight_decay, float grad_scale,
+                              hipStream_t stream) {
+    TraceRange range("train_step");
+    synced_gradients(x, target, batch, stream);
     optimizer_step(lr, momentum, weight_decay, grad_scale, stream);
+}
+
+void VggEngineF32::gradients_step(const float* x, const int64_t* target, int batch,
+                                  hipStream_t stream) {
+    TraceRange range("train_step");
+    synced_gradients(x, target, batch, stream);
+    if (reducer_) reducer_->wait_all(stream);
+}
+
+void VggEngineF32::parameters_updated(hipStream_t stream) {
+    const float* bsrc = nullptr; float* bdst = nullptr; size_t bn = 0;
+    if (reducer_ && reducer_->take_pending_buffers(&bsrc, &bdst, &bn))
+        check_hip(hipMemcpyAsync(bdst, bsrc, bn * sizeof(float), hipMemcpyDeviceToDevice, stream),
+                  "hipMemcpyAsync(buffers)");
+    refresh_weights(stream);
 }
 
 void VggEngineF32::eval_step(const float* x, const int64_t* target, int batch, hipStream_t stream) {
@@ -562,6 +582,10 @@ void bind_engine_f32(py::module_& m) {
         .def("forward_backward", [](VggEngineF32& e, uintptr_t x, uintptr_t t, int batch, uintptr_t s) {
             e.forward_backward((const float*)x, (const int64_t*)t, batch, (hipStream_t)s);
         })
+        .def("gradients_step", [](VggEngineF32& e, uintptr_t x, uintptr_t t, int batch, uintptr_t s) {
+            e.gradients_step((const float*)x, (const int64_t*)t, batch, (hipStream_t)s);
+        })
+        .def("parameters_updated", [](VggEngineF32& e, uintptr_t s) { e.parameters_updated((hipStream_t)s); })
         .def("optimizer_step", [](VggEngineF32& e, float lr, float mu, float wd, float gs, uintptr_t s) {
             e.optimizer_step(lr, mu, wd, gs, (hipStream_t)s);
         })

@@ -124,6 +124,11 @@ class VggEngine {
     // if one is attached (set_manual_sync), optimizer_step.
     void train_step(const uint16_t* x_nhwc4, const int64_t* target, int batch, float lr,
                     float momentum, float weight_decay, float grad_scale, hipStream_t stream);
+    // The same iteration for an optimizer outside the engine: everything of train_step up to the
+    // update (afterwards `stream` has the final gradients), then - once the caller has enqueued its
+    // update of the bound parameters - the buffers and weight layouts that follow from it.
+    void gradients_step(const uint16_t* x_nhwc4, const int64_t* target, int batch, hipStream_t stream);
+    void parameters_updated(hipStream_t stream);
     void set_manual_sync(ManualSync* sync) { manual_sync_ = sync; }
     // forward only (evaluation statistics); accumulates loss / correct into the eval slots
     void eval_step(const uint16_t* x_nhwc4, const int64_t* target, int batch, hipStream_t stream);
@@ -167,6 +172,7 @@ class VggEngine {
         size_t gout_off;                              // arena: dL/d(conv output), read by dgrad + wgrad
     };
     void backward(const uint16_t* x_nhwc4, const int64_t* target, int batch, hipStream_t stream);
+    void synced_gradients(const uint16_t* x_nhwc4, const int64_t* target, int batch, hipStream_t stream);
     void fire_buckets(int layer, hipStream_t stream);
     void flush_wgrad_sums(hipStream_t stream);
     void join_wgrad_stream(hipStream_t stream);
@@ -289,6 +295,8 @@ class VggEngineF32 {
                         hipStream_t stream);
     void train_step(const float* x_nhwc4, const int64_t* target, int batch, float lr,
                     float momentum, float weight_decay, float grad_scale, hipStream_t stream);
+    void gradients_step(const float* x_nhwc4, const int64_t* target, int batch, hipStream_t stream);
+    void parameters_updated(hipStream_t stream);
     void eval_step(const float* x_nhwc4, const int64_t* target, int batch, hipStream_t stream);
     // Weight gradients (with bias gradients, slab sums and the buckets they complete) on a second
     // HIP stream next to the pool / BatchNorm / backward-data chain, one event per layer; the
@@ -308,6 +316,7 @@ class VggEngineF32 {
     ~VggEngineF32();
 
   private:
+    void synced_gradients(const float* x_nhwc4, const int64_t* target, int batch, hipStream_t stream);
     struct Buffers {
         size_t wd_off = 0, pre_off = 0, out_off = 0, pool_off = 0, gout_off = 0;   // arena
         // arena: a transit buffer of the layer's own for the gradient arriving from the next

@@ -17,9 +17,11 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
-from ..config import SYNC_ALL_REDUCE, SYNC_DDP, SYNC_GATHER_SCATTER, SYNC_NONE, TrainConfig
+from ..config import (OPT_MUON, SYNC_ALL_REDUCE, SYNC_DDP, SYNC_GATHER_SCATTER, SYNC_NONE,
+                      TrainConfig)
 from ..models.vgg import VGG, VGG_WIDTHS
 from ..ops import native
+from ..optim.muon import split_slots
 from ..parallel.comm import Communicator
 from ..parallel.flat import cap_tail_bucket
 
@@ -40,6 +42,9 @@ class NativeBackend:
         self.loader_layout = "nhwc4_fp32" if self.fp32 else "nhwc4_bf16"
         if self.fp32 and cfg.use_graph:
             raise ValueError("--graph replays the bf16 engine's step; the fp32 engine has no "
+                             "graph mode")
+        if cfg.optimizer == OPT_MUON and cfg.use_graph:
+            raise ValueError("--graph replays the engine's own SGD step; --optimizer muon has no "
                              "graph mode")
         self.cfg = cfg
         self.device = device
@@ -77,6 +82,11 @@ class NativeBackend:
         self._loss_off = e.loss_offset
         self._loss_view = self.workspace[e.loss_offset:e.loss_offset + 1]
         self._training = True
+        self._muon = self._muon_ws = None
+        if cfg.optimizer == OPT_MUON:
+            matrices, segments = split_slots(self.slots, None, "original")
+            self._muon = native.MuonPlan(matrices, segments, precision=cfg.muon_precision)
+            self._muon_ws = torch.empty(self._muon.workspace_bytes, dtype=torch.uint8, device=device)
         # initial weights: the stock module's initialisers under the caller's seed, so every
         # backend (and every rank) starts from the same numbers the reference would
         if init_state is None:
@@ -106,7 +116,8 @@ class NativeBackend:
             # the optimizer update can run inside backward when the gradients backward leaves
             # behind are final: no sync, or the bucket reducer (the two manual modes
             # synchronise after backward has ended)
-            self._fuse_opt = bool(cfg.fused_optimizer) and e.wgrad_overlap and self.manual is None
+            self._fuse_opt = bool(cfg.fused_optimizer) and e.wgrad_overlap and \
+                self.manual is None and self._muon is None
             # deep layers' update on the side stream, next to the first layers of the next forward
             late = int(os.environ.get("DML_UPDATE_OVERLAP", cfg.update_overlap))
             if late < 0:        # auto: from the first layer of the last spatial sizes (4x4 and below)
@@ -217,7 +228,7 @@ class NativeBackend:
                 # staging floats the first bucket's slice ends with (see BucketReducer)
                 self.reducer.set_buffer_sync(self.bn_buffers.data_ptr(),
                                              self.grads[e.param_elems:].data_ptr(), e.bn_elems)
-            if cfg.grad_comm_dtype == "bf16" and not self.fp32:
+            if cfg.grad_comm_dtype == "bf16" and not self.fp32 and self._muon is None:
                 # the fused update reads the reduced bf16 values where the collective left them
                 # (no widening pass; ``grads`` keeps this rank's own gradients)
                 self.reducer.set_keep_on_wire(True)
@@ -351,6 +362,14 @@ class NativeBackend:
                                   self._grad_scale)
         if cfg.use_graph and self.world == 1:
             return self._train_step_graph(data, target, n, s)
+        if self._muon is not None:
+            e.gradients_step(data.data_ptr(), target.data_ptr(), n, s)
+            native.muon_step_(self._muon, self._params, self.grads[:self._params.numel()],
+                              self._momentum, cfg.muon_lr, cfg.muon_momentum, cfg.muon_weight_decay,
+                              True, cfg.lr, cfg.momentum, cfg.weight_decay, self._grad_scale,
+                              self._muon_ws)
+            e.parameters_updated(s)
+            return self._loss_view
         e.train_step(data.data_ptr(), target.data_ptr(), n, cfg.lr, cfg.momentum, cfg.weight_decay,
                      self._grad_scale, s)
         return self._loss_view

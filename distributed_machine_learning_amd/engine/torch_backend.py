@@ -14,8 +14,10 @@ from typing import Dict, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from ..config import SYNC_ALL_REDUCE, SYNC_DDP, SYNC_GATHER_SCATTER, SYNC_NONE, TrainConfig
+from ..config import (OPT_MUON, SYNC_ALL_REDUCE, SYNC_DDP, SYNC_GATHER_SCATTER, SYNC_NONE,
+                      TrainConfig)
 from ..models.vgg import VGG
+from ..optim.muon import Muon
 from ..parallel.comm import Communicator
 from ..parallel.flat import FlatModule
 from ..parallel.strategies import (AllReduceSync, BucketedSync, GatherScatterSync, GradSync,
@@ -48,8 +50,14 @@ class TorchBackend:
         self.model = VGG(cfg.arch, cfg.batch_norm, cfg.num_classes).to(device)
         self.flat = FlatModule(self.model)
         self.flat.params.grad = self.flat.grads
-        self.optimizer = torch.optim.SGD([self.flat.params], lr=cfg.lr, momentum=cfg.momentum,
-                                         weight_decay=cfg.weight_decay)
+        if cfg.optimizer == OPT_MUON:
+            self.optimizer = Muon(self.flat, lr=cfg.muon_lr, momentum=cfg.muon_momentum,
+                                  weight_decay=cfg.muon_weight_decay, precision=cfg.muon_precision,
+                                  sgd_lr=cfg.lr, sgd_momentum=cfg.momentum,
+                                  sgd_weight_decay=cfg.weight_decay)
+        else:
+            self.optimizer = torch.optim.SGD([self.flat.params], lr=cfg.lr, momentum=cfg.momentum,
+                                             weight_decay=cfg.weight_decay)
         self.sync = build_sync(cfg, comm, self.flat)
         self.bf16 = cfg.dtype == "bf16"
 
