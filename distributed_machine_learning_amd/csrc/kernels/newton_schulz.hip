@@ -337,19 +337,41 @@ struct TileTimes {
     double tile[3], tile_more[3];       // GRAM, SQUARE, APPLY
 };
 struct BigTile {        // 8 waves of 64 x 64, two stages in flight
+    static constexpr bool kRing = true;
+    static constexpr int kGroups = 1;
     static constexpr int kM = 128, kN = 256, kWavesM = 2, kWavesN = 4, kStages = 3, kBlocksPerCu = 1;
     static constexpr bool kTurns = true;
     static constexpr TileTimes kTimes = {1.0, 0.85, 0.0, {15, 20, 14}, {0, 0, 0}};
 };
 struct MidTile {        // 4 waves of 64 x 64, one stage in flight
+    static constexpr bool kRing = true;
+    static constexpr int kGroups = 1;
     static constexpr int kM = 128, kN = 128, kWavesM = 2, kWavesN = 2, kStages = 2, kBlocksPerCu = 2;
     static constexpr bool kTurns = false;
     static constexpr TileTimes kTimes = {0.85, 0.7, 0.25, {8, 12, 8}, {0, 0, 0}};
 };
 struct SmallTile {      // 4 waves of 32 x 32, two stages in flight
+    static constexpr bool kRing = true;
+    static constexpr int kGroups = 1;
     static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 3, kBlocksPerCu = 3;
     static constexpr bool kTurns = false;
     static constexpr TileTimes kTimes = {0.2, 0.18, 0.13, {4, 5, 3}, {1.5, 2, 1}};
+};
+
+// Where tiles are few, a CU's only block takes two steps at once: 0.25 us a step against 0.33 with one
+// group (three SmallTile blocks on a CU: 0.2).
+struct PairTile {       // two groups of 4 waves of 32 x 32, each with half of the summed index
+    static constexpr bool kRing = true;
+    static constexpr int kGroups = 2;
+    static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 3, kBlocksPerCu = 1;
+    static constexpr bool kTurns = false;
+    static constexpr TileTimes kTimes = {0.5, 0.46, 0.0, {4.8, 5, 3.5}, {0, 0, 0}};
+};
+struct ShortTile {      // 8 waves, each with an eighth of the summed index; a step is 8 x 64 of it
+    static constexpr int kM = 32, kN = 32, kWaves = 8, kBlocksPerCu = 2;
+    static constexpr bool kRing = false;
+    static constexpr int kGroups = 1;
+    static constexpr TileTimes kTimes = {2.0, 0.3, 1.5, {2.5, 3, 0}, {0.5, 0.5, 0}};
 };
 
 // This wave's loads but the last N have landed and its LDS reads are done, then so for all waves.
@@ -660,22 +682,24 @@ struct NsSides {
 //     eight rows that half a wave reads at once meet different banks.
 // The columns' operand is the first of the MFMA, so a lane ends with four consecutive columns of a row.
 template <typename G, bool WIDE, int PHASE, typename OUT>
-__global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void ns_product_kernel(
+__global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void ns_product_kernel(
     NsTable tab, char* ws, float* slab, NsStep s, NsResult res) {
-    constexpr int kThreads = G::kWavesM * G::kWavesN * 64, kWaves = kThreads / 64;
+    constexpr int kWaves = G::kWavesM * G::kWavesN, kThreads = G::kGroups * kWaves * 64;
     constexpr int WM = G::kM / G::kWavesM, WN = G::kN / G::kWavesN, FM = WM / 16, FN = WN / 16;
     constexpr int kStage = (G::kM + G::kN) * 128, LD = G::kN + 4;
-    constexpr int kRing = G::kStages * kStage, kTile = G::kM * LD * 4;
+    constexpr int kRing = G::kStages * kStage, kRings = G::kGroups * kRing, kTile = G::kM * LD * 4;
     constexpr int kLoads = kStage / 1024 / kWaves;      // per wave and stage
     constexpr int kStep = WIDE ? 32 : 64;
-    __shared__ __attribute__((aligned(1024))) char smem[kRing > kTile ? kRing : kTile];
+    __shared__ __attribute__((aligned(1024))) char smem[kRings > kTile ? kRings : kTile];
     __shared__ float rows[G::kM], cols[G::kN];
     static_assert(kThreads >= G::kM && kThreads >= G::kN, "one thread per row and column");
 
     const NsItem it = item_of<G, PHASE>(tab, blockIdx.x, gridDim.x);
     const NsProblem& q = tab.p[it.problem];
     const NsPlanes w = ns_planes(q, ws, it.b, s.buffer);
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int group = G::kGroups > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / kWaves : 0;
+    const int wave = (threadIdx.x >> 6) - group * kWaves, lane = threadIdx.x & 63;
+    char* ring = smem + group * kRing;
     const int i0 = it.ti * G::kM, j0 = it.tj * G::kN;
     // rows' operand, columns' operand
     const uint16_t* rp = PHASE == GRAM ? w.y : w.square(s.x);
@@ -692,7 +716,13 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
         from = (int)((long long)all * it.split / q.splits);
         to = (int)((long long)all * (it.split + 1) / q.splits);
     }
-    const int steps = to - from;
+    // `mine` of the steps are this group's; a group may have one less than another
+    const int steps = (to - from + G::kGroups - 1) / G::kGroups;
+    int mine = steps;
+    if (G::kGroups > 1) {
+        from += group * steps;
+        mine = min(steps, to - from);
+    }
 
     // Addresses of this lane's pieces in the first stage; a stage on, they move by a fixed distance.
     const char* src[kLoads];
@@ -726,7 +756,7 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
         }
     }
     auto stage = [&](int n) {
-        char* dst = smem + (n % G::kStages) * kStage;
+        char* dst = ring + (n % G::kStages) * kStage;
 #pragma unroll
         for (int l = 0; l < kLoads; ++l) {
             const int kb = wave + l * kWaves;
@@ -749,15 +779,15 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
 #pragma unroll
         for (int y = 0; y < FN; ++y) {
             const int pair = ((wj + y * 16) >> 4) ^ pair_swizzle<G::kN>(row);
-            across[y] = (unsigned)(size_t)(lds_char*)smem + G::kM * 128 + row * (G::kN * 2) + pair * 32 + (l15 & 3) * 8;
+            across[y] = (unsigned)(size_t)(lds_char*)ring + G::kM * 128 + row * (G::kN * 2) + pair * 32 + (l15 & 3) * 8;
         }
     }
 #pragma unroll
     for (int n = 0; n < G::kStages - 1; ++n)
-        if (n < steps) stage(n);
+        if (n < mine) stage(n);
     struct Fragments { f16x8 r[2][FM], c[2][FN]; };
     auto read = [&](int k, Fragments& f) {
-        const char* sr = smem + (k % G::kStages) * kStage;
+        const char* sr = ring + (k % G::kStages) * kStage;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -793,7 +823,7 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
                         f.c[WIDE ? n >> 1 : n][y], f.r[WIDE ? n & 1 : n][x], acc[x][y], 0, 0, 0);
     };
     auto await = [&](int k) {
-        if (k + G::kStages - 2 < steps) await_stage<(G::kStages - 2) * kLoads>();
+        if (k + G::kStages - 2 < mine) await_stage<(G::kStages - 2) * kLoads>();
         else await_stage<0>();
     };
     if constexpr (G::kTurns) {
@@ -818,16 +848,16 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
         // A wave reads the fragments of a step while the products of the step before run.  All waves
         // have read stage k when they pass the barrier of step k, so it is refilled at once.
         Fragments f0, f1;
-        if (G::kStages - 1 < steps) stage(G::kStages - 1);
+        if (G::kStages - 1 < mine) stage(G::kStages - 1);
         await(0);
         read(0, f0);
         auto step = [&](int k, const Fragments& now, Fragments& next) {
             if (k + 1 < steps) {
                 await(k + 1);
-                if (k + G::kStages < steps) stage(k + G::kStages);
+                if (k + G::kStages < mine) stage(k + G::kStages);
                 read(k + 1, next);
             }
-            multiply(now);
+            if (G::kGroups == 1 || k < mine) multiply(now);
         };
         for (int k = 0; k < steps; k += 2) {
             step(k, f0, f1);
@@ -837,12 +867,25 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
         Fragments f;
         for (int k = 0; k < steps; ++k) {
             await(k);
-            if (k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
+            if (k + G::kStages - 1 < mine) stage(k + G::kStages - 1);
             read(k, f);
-            multiply(f);
+            if (G::kGroups == 1 || k < mine) multiply(f);
         }
     }
+    if constexpr (G::kGroups == 2) {        // the second group's sums to the first
+        static_assert(kWaves * FM * FN * 1024 <= kRing, "the sums fit the first ring");
+        f32x4* over = (f32x4*)smem + (wave * FM * FN) * 64 + lane;
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < FM * FN; ++x)
+            if (group) over[x * 64] = acc[x / FN][x % FN];
+        __syncthreads();
+#pragma unroll
+        for (int x = 0; x < FM * FN; ++x)
+            if (!group) acc[x / FN][x % FN] += over[x * 64];
+    }
     if (it.split >= 0) {        // fragments of 16 x 16, lane by lane
+        if (group) return;
         float* to_slab = slab + (size_t)it.slab * G::kM * G::kN;
 #pragma unroll
         for (int x = 0; x < FM; ++x)
@@ -855,11 +898,12 @@ __global__ __launch_bounds__(G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void
     auto put = [&]() {
         sides.put(rows, cols);
         __syncthreads();        // the ring's last stage has been read
+        if (group == 0)
 #pragma unroll
-        for (int x = 0; x < FM; ++x)
+            for (int x = 0; x < FM; ++x)
 #pragma unroll
-            for (int y = 0; y < FN; ++y)
-                *(f32x4*)(E + (wi + x * 16 + l15) * LD + wj + y * 16 + lq * 4) = acc[x][y] * s.inv;
+                for (int y = 0; y < FN; ++y)
+                    *(f32x4*)(E + (wi + x * 16 + l15) * LD + wj + y * 16 + lq * 4) = acc[x][y] * s.inv;
         __syncthreads();
     };
     ns_epilogue<G::kM, G::kN, LD, kThreads, G::kM, PHASE, OUT>(E, rows, cols, q, w, ws, it.b, i0, j0, s, res, put);
@@ -915,6 +959,107 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, con
         __syncthreads();
     };
     ns_epilogue<64, 64, LD, 256, G::kM, PHASE, OUT>(E, rows, cols, q, w, ws, b, i0, j0, s, res, put);
+}
+
+// The symmetric products where their sums are short.  A 64 x 64 tile of 512 summed values spends its
+// time on 16 barriers one after another; here the 8 waves of a block take 64 of the summed values each,
+// straight from memory to registers with every load in flight at once, and add their 32 x 32 parts in
+// LDS, in the order of the waves: 8.5 us instead of 13 for 512 x 512.  Each operand is read twice as
+// often as by 64 x 64 tiles, and that bounds it from about 700 values on (777 x 777: 18 us, PairTile 14).
+template <bool WIDE, int PHASE>
+__global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsTable tab, char* ws, NsStep s) {
+    static_assert(PHASE == GRAM || PHASE == SQUARE, "operands along the summed index");
+    typedef ShortTile G;
+    constexpr int LD = 36, kPlanes = WIDE ? 2 : 1;
+    __shared__ __attribute__((aligned(16))) f32x4 parts[G::kWaves][256];
+    __shared__ __attribute__((aligned(16))) float E[32 * LD];
+    const NsItem it = item_of<G, PHASE>(tab, blockIdx.x, gridDim.x);
+    const NsProblem& q = tab.p[it.problem];
+    const NsPlanes w = ns_planes(q, ws, it.b, s.buffer);
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63, l15 = lane & 15, lq = lane >> 4;
+    const int i0 = it.ti * 32, j0 = it.tj * 32;
+    const uint16_t* rp = PHASE == GRAM ? w.y : w.square(s.x);
+    const uint16_t* cp = PHASE == GRAM ? w.y : w.square(s.w);
+    const size_t plane = PHASE == GRAM ? w.yplane : w.aplane;
+    const int ld = PHASE == GRAM ? w.yld : w.ald, depth = PHASE == GRAM ? q.np : q.mp;
+
+    // of the first four waves, thread t finishes row fr, columns fc .. fc + 3 (as its accumulators lie)
+    const int fr = (t >> 7 & 1) * 16 + l15, fc = (t >> 6 & 1) * 16 + lq * 4;
+    uint2 xh, xl, wh, wl;
+    float dx = 0.f;
+    f32x4 dw;
+    if (PHASE == SQUARE && t < 256) {
+        const size_t at = (size_t)(i0 + fr) * ld + j0 + fc;
+        xh = *(const uint2*)(rp + at);
+        xl = *(const uint2*)(rp + plane + at);
+        wh = *(const uint2*)(cp + at);
+        wl = *(const uint2*)(cp + plane + at);
+        dx = w.diagonal(s.x)[i0 + fr];
+        dw = *(const f32x4*)(w.diagonal(s.w) + j0 + fc);
+    }
+    f32x4 acc[2][2] = {};
+    for (int k = wave * 64; k < depth; k += G::kWaves * 64) {
+        f16x8 r[2][2][kPlanes], c[2][2][kPlanes];       // half of the 64 values, 16 rows, plane
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int l = 0; l < kPlanes; ++l) {
+                    const size_t in = (size_t)l * plane + k + h * 32 + lq * 8;
+                    r[h][x][l] = *(const f16x8*)(rp + (size_t)(i0 + x * 16 + l15) * ld + in);
+                    c[h][x][l] = *(const f16x8*)(cp + (size_t)(j0 + x * 16 + l15) * ld + in);
+                }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][0], r[h][x][0], acc[x][y], 0, 0, 0);
+                    if constexpr (WIDE) {
+                        acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][0], r[h][x][1], acc[x][y], 0, 0, 0);
+                        acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][1], r[h][x][0], acc[x][y], 0, 0, 0);
+                    }
+                }
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) parts[wave][(x * 2 + y) * 64 + lane] = acc[x][y];
+    __syncthreads();
+    if (t < 256) {
+        f32x4 z = parts[0][t];
+#pragma unroll
+        for (int k = 1; k < G::kWaves; ++k) z += parts[k][t];
+        z *= s.inv;
+        const int gi = i0 + fr, gj = j0 + fc;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (PHASE == SQUARE) {
+                const float o = (f16_value(((const uint16_t*)&wh)[j]) + f16_value(((const uint16_t*)&wl)[j])) * s.iw;
+                const float x = (f16_value(((const uint16_t*)&xh)[j]) + f16_value(((const uint16_t*)&xl)[j])) * s.ix;
+                z[j] = gi == gj + j ? s.k1 * (z[j] + dx * dw[j]) + (s.k2 * dw[j] + s.k0)
+                                    : s.k1 * (z[j] + (dx * o + x * dw[j])) + s.k2 * o;
+            }
+            if (gi == gj + j) {
+                w.diagonal(s.z)[gi] = z[j];
+                z[j] = 0.f;
+            }
+        }
+        *(f32x4*)(E + fr * LD + fc) = z * s.sz;
+    }
+    __syncthreads();
+    // the first four waves write the tile, the others its mirror image
+    const bool mirror = t >= 256;
+    if (mirror && i0 == j0) return;
+    const int r = (t & 255) >> 3, c = (t & 7) * 4;
+    uint16_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split_f16(mirror ? E[(c + j) * LD + r] : E[r * LD + c + j], hi[j], lo[j]);
+    uint16_t* at = w.square(s.z) + (size_t)((mirror ? j0 : i0) + r) * w.ald + (mirror ? i0 : j0) + c;
+    *(uint2*)at = *(const uint2*)hi;
+    *(uint2*)(at + w.aplane) = *(const uint2*)lo;
 }
 
 // ------------------------------------------------------------------ one block per matrix
@@ -1203,7 +1348,7 @@ int scale_exp(double v) {
 struct NsLaunch {
     NsTable tab, join;          // `join`: the split entries, counted in tiles
     unsigned blocks = 0, join_tiles = 0;
-    int tile = 0;               // 0 big, 1 mid, 2 small
+    int tile = 0;               // 0 big, 1 mid, 2 small, 3 pair, 4 short
     double cost = 0;            // estimate, us
     size_t slab_bytes = 0;
 
@@ -1245,7 +1390,10 @@ struct NsLaunch {
         std::vector<Entry> whole, split;
         long long total = 0;
         int longest = 0;
-        auto steps_of = [&](const NsProblem& p) { return (phase == GRAM ? p.np : p.mp) / step; };
+        auto steps_of = [&](const NsProblem& p) {
+            const int depth = phase == GRAM ? p.np : p.mp;
+            return G::kRing ? depth / step : (depth + 511) / 512;
+        };
         for (const NsProblem& p : ps) {
             total += checked(tiles_of<G>(p, phase)) * (long long)p.batch;
             longest = std::max(longest, steps_of(p));
@@ -1254,28 +1402,32 @@ struct NsLaunch {
         auto round_us = [&](long long blocks, double steps, double finish) {
             const TileTimes& t = G::kTimes;
             const double n = (double)std::min<long long>(G::kBlocksPerCu, (blocks + kCus - 1) / kCus);
-            return steps * ((wide ? t.wide_step : t.narrow_step) + t.step_more * n) +
+            return steps / G::kGroups * ((wide ? t.wide_step : t.narrow_step) + t.step_more * n) +
                    finish * (t.tile[phase] + t.tile_more[phase] * n);
         };
-        // the joining launch: its latency, and the parts written and read at 4 TB/s
-        auto join_us = [&](long long items) { return 9.0 + (double)items * G::kM * G::kN * 8 / 4e6; };
+        // the joining launch: its latency, a tile's parts, and all parts written and read at 4 TB/s
+        auto join_us = [&](long long items, int parts) {
+            return (phase == SQUARE ? 8.5 : 7.0) + 0.2 * parts + (double)items * G::kM * G::kN * 8 / 4e6;
+        };
         const long long rest = total % kSlots;
         const double full = (total / kSlots) * round_us(kSlots, longest, 1);
         long long keep = total;         // tiles that stay whole
         cost = full + (rest ? round_us(rest, longest, 1) : 0);
-        if (rest && rest * 4 <= kSlots * 3) {
+        if (G::kRing && rest && rest * 4 <= kSlots * 3) {
             if (total < kSlots) {       // one round: parts of equal length, of all that are longer
                 int part = longest;
-                long long items = total;
                 for (int n = kShortest; n < longest; ++n) {
-                    items = 0;
+                    long long items = 0;
                     for (const NsProblem& p : ps)
                         items += tiles_of<G>(p, phase) * p.batch * ((steps_of(p) + n - 1) / n);
-                    if (items <= kSlots) { part = n; break; }
+                    if (items > kSlots) continue;
+                    const double divided = round_us(items, n, 0.5) + join_us(items, (longest + n - 1) / n);
+                    if (divided < cost) {
+                        cost = divided;
+                        part = n;
+                    }
                 }
-                const double divided = round_us(items, part, 0.5) + join_us(items);
-                if (part < longest && divided < cost) {
-                    cost = divided;
+                if (part < longest) {
                     keep = 0;
                     for (const NsProblem& p : ps) {
                         const long long n = tiles_of<G>(p, phase) * p.batch;
@@ -1286,7 +1438,7 @@ struct NsLaunch {
             } else {
                 const int parts = (int)std::min<long long>(kSlots / rest, steps_of(ps.back()) / kShortest);
                 if (parts > 1) {
-                    const double divided = full + round_us(rest * parts, (double)longest / parts, 0.5) + join_us(rest * parts);
+                    const double divided = full + round_us(rest * parts, (double)longest / parts, 0.5) + join_us(rest * parts, parts);
                     if (divided < cost) {
                         cost = divided;
                         keep = total - rest;
@@ -1332,11 +1484,12 @@ struct NsLaunch {
         return l;
     }
     static NsLaunch product(const std::vector<NsProblem>& ps, int phase, bool wide) {
-        double cost[3];
-        NsLaunch l[3] = {tiled<BigTile>(ps, phase, wide, cost[0]), tiled<MidTile>(ps, phase, wide, cost[1]),
-                         tiled<SmallTile>(ps, phase, wide, cost[2])};
+        double cost[5];
+        NsLaunch l[5] = {tiled<BigTile>(ps, phase, wide, cost[0]), tiled<MidTile>(ps, phase, wide, cost[1]),
+                         tiled<SmallTile>(ps, phase, wide, cost[2]), tiled<PairTile>(ps, phase, wide, cost[3]), {}};
+        if (phase != APPLY) l[4] = tiled<ShortTile>(ps, phase, wide, cost[4]);
         int best = 0;
-        for (int i = 0; i < 3; ++i) {
+        for (int i = 0; i < (phase == APPLY ? 4 : 5); ++i) {
             l[i].tile = i;
             if (cost[i] < cost[best]) best = i;
         }
@@ -1570,7 +1723,7 @@ template <typename G, bool WIDE, int PHASE, typename OUT>
 void launch_product(const NsLaunch& l, char* ws, float* slab, const NsStep& s, const NsResult& r,
                     hipStream_t stream) {
     hipLaunchKernelGGL((ns_product_kernel<G, WIDE, PHASE, OUT>), dim3(l.blocks),
-                       dim3(G::kWavesM * G::kWavesN * 64), 0, stream, l.tab, ws, slab, s, r);
+                       dim3(G::kGroups * G::kWavesM * G::kWavesN * 64), 0, stream, l.tab, ws, slab, s, r);
     if (l.join_tiles)
         hipLaunchKernelGGL((ns_join_kernel<G, PHASE, OUT>), dim3(l.join_tiles * (G::kM / 64) * (G::kN / 64)),
                            dim3(256), 0, stream, l.join, ws, slab, s, r);
@@ -1583,6 +1736,14 @@ void launch_phase(const NsLaunch& l, int phase, NsType type, char* ws, float* sl
     else if (type == NS_BF16) launch_product<G, WIDE, APPLY, bf16_t>(l, ws, slab, s, r, stream);
     else if (type == NS_F16) launch_product<G, WIDE, APPLY, f16_t>(l, ws, slab, s, r, stream);
     else launch_product<G, WIDE, APPLY, float>(l, ws, slab, s, r, stream);
+}
+
+void launch_short(const NsLaunch& l, int phase, bool wide, char* ws, const NsStep& s, hipStream_t stream) {
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(l.blocks), dim3(ShortTile::kWaves * 64), 0, stream, l.tab, ws, s);
+    };
+    if (phase == GRAM) go(wide ? ns_short_kernel<true, GRAM> : ns_short_kernel<false, GRAM>);
+    else go(wide ? ns_short_kernel<true, SQUARE> : ns_short_kernel<false, SQUARE>);
 }
 
 }  // namespace
@@ -1612,14 +1773,17 @@ void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, cons
         prepare(*g, (double*)(ws + partials_), std::ldexp(1.f, x_exp_));
         for (const auto& op : ops_) {
             const NsLaunch& l = g->product[op->phase];
+            const bool wide = op->phase == SQUARE ? squares_wide_ : wide_;
             auto go = [&](auto tile) {
                 typedef decltype(tile) G;
-                if (op->phase == SQUARE ? squares_wide_ : wide_) launch_phase<G, true>(l, op->phase, type, ws, slab, op->step, r, stream);
+                if (wide) launch_phase<G, true>(l, op->phase, type, ws, slab, op->step, r, stream);
                 else launch_phase<G, false>(l, op->phase, type, ws, slab, op->step, r, stream);
             };
             if (l.tile == 0) go(BigTile{});
             else if (l.tile == 1) go(MidTile{});
-            else go(SmallTile{});
+            else if (l.tile == 2) go(SmallTile{});
+            else if (l.tile == 3) go(PairTile{});
+            else launch_short(l, op->phase, wide, ws, op->step, stream);
         }
     }
 }
