@@ -336,23 +336,33 @@ struct TileTimes {
     double wide_step, narrow_step, step_more;
     double tile[3], tile_more[3];       // GRAM, SQUARE, APPLY
 };
+// Only for narrow B Y: 149 us for 4096 x 4096, BigTile 169, since it reads three quarters as much LDS for
+// a product.  Wide it is the slower one (8192 x 2048, four of them: 1613 us against 1529), and the
+// symmetric products have too few tiles of this size and more epilogue than registers.
+struct HugeTile {       // 8 waves of 128 x 64 in two halves, one stage in flight
+    static constexpr bool kRing = true;
+    static constexpr int kGroups = 1, kParts = 2;
+    static constexpr int kM = 256, kN = 256, kWavesM = 2, kWavesN = 4, kStages = 2, kBlocksPerCu = 1;
+    static constexpr bool kTurns = true;
+    static constexpr TileTimes kTimes = {0, 1.55, 0.0, {0, 0, 20}, {0, 0, 0}};
+};
 struct BigTile {        // 8 waves of 64 x 64, two stages in flight
     static constexpr bool kRing = true;
-    static constexpr int kGroups = 1;
+    static constexpr int kGroups = 1, kParts = 1;
     static constexpr int kM = 128, kN = 256, kWavesM = 2, kWavesN = 4, kStages = 3, kBlocksPerCu = 1;
     static constexpr bool kTurns = true;
     static constexpr TileTimes kTimes = {1.0, 0.85, 0.0, {15, 20, 14}, {0, 0, 0}};
 };
 struct MidTile {        // 4 waves of 64 x 64, one stage in flight
     static constexpr bool kRing = true;
-    static constexpr int kGroups = 1;
+    static constexpr int kGroups = 1, kParts = 1;
     static constexpr int kM = 128, kN = 128, kWavesM = 2, kWavesN = 2, kStages = 2, kBlocksPerCu = 2;
     static constexpr bool kTurns = false;
     static constexpr TileTimes kTimes = {0.85, 0.7, 0.25, {8, 12, 8}, {0, 0, 0}};
 };
 struct SmallTile {      // 4 waves of 32 x 32, two stages in flight
     static constexpr bool kRing = true;
-    static constexpr int kGroups = 1;
+    static constexpr int kGroups = 1, kParts = 1;
     static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 3, kBlocksPerCu = 3;
     static constexpr bool kTurns = false;
     static constexpr TileTimes kTimes = {0.2, 0.18, 0.13, {4, 5, 3}, {1.5, 2, 1}};
@@ -362,7 +372,7 @@ struct SmallTile {      // 4 waves of 32 x 32, two stages in flight
 // group (three SmallTile blocks on a CU: 0.2).
 struct PairTile {       // two groups of 4 waves of 32 x 32, each with half of the summed index
     static constexpr bool kRing = true;
-    static constexpr int kGroups = 2;
+    static constexpr int kGroups = 2, kParts = 1;
     static constexpr int kM = 64, kN = 64, kWavesM = 2, kWavesN = 2, kStages = 3, kBlocksPerCu = 1;
     static constexpr bool kTurns = false;
     static constexpr TileTimes kTimes = {0.5, 0.46, 0.0, {4.8, 5, 3.5}, {0, 0, 0}};
@@ -370,7 +380,7 @@ struct PairTile {       // two groups of 4 waves of 32 x 32, each with half of t
 struct ShortTile {      // 8 waves, each with an eighth of the summed index; a step is 8 x 64 of it
     static constexpr int kM = 32, kN = 32, kWaves = 8, kBlocksPerCu = 2;
     static constexpr bool kRing = false;
-    static constexpr int kGroups = 1;
+    static constexpr int kGroups = 1, kParts = 1;
     static constexpr TileTimes kTimes = {2.0, 0.3, 1.5, {2.5, 3, 0}, {0.5, 0.5, 0}};
 };
 
@@ -685,9 +695,12 @@ template <typename G, bool WIDE, int PHASE, typename OUT>
 __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void ns_product_kernel(
     NsTable tab, char* ws, float* slab, NsStep s, NsResult res) {
     constexpr int kWaves = G::kWavesM * G::kWavesN, kThreads = G::kGroups * kWaves * 64;
+    static_assert(G::kParts == 1 || G::kParts == G::kWavesM, "a part of the rows is a row of waves");
     constexpr int WM = G::kM / G::kWavesM, WN = G::kN / G::kWavesN, FM = WM / 16, FN = WN / 16;
     constexpr int kStage = (G::kM + G::kN) * 128, LD = G::kN + 4;
-    constexpr int kRing = G::kStages * kStage, kRings = G::kGroups * kRing, kTile = G::kM * LD * 4;
+    constexpr int kRing = G::kStages * kStage, kRings = G::kGroups * kRing;
+    constexpr int kRows = G::kM / G::kParts, kTile = kRows * LD * 4;      // rows that are finished at a time
+    constexpr int FP = FM / G::kParts;
     constexpr int kLoads = kStage / 1024 / kWaves;      // per wave and stage
     constexpr int kStep = WIDE ? 32 : 64;
     __shared__ __attribute__((aligned(1024))) char smem[kRings > kTile ? kRings : kTile];
@@ -785,16 +798,17 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
 #pragma unroll
     for (int n = 0; n < G::kStages - 1; ++n)
         if (n < mine) stage(n);
-    struct Fragments { f16x8 r[2][FM], c[2][FN]; };
-    auto read = [&](int k, Fragments& f) {
+    struct Fragments { f16x8 r[2][FP], c[2][FN]; };
+    auto read = [&](int k, int part, Fragments& f) {
         const char* sr = ring + (k % G::kStages) * kStage;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int x = 0; x < FM; ++x) {
-                const int r = wi + x * 16 + l15;
+            for (int x = 0; x < FP; ++x) {
+                const int r = wi + (part * FP + x) * 16 + l15;
                 f.r[h][x] = *(const f16x8*)(sr + r * 128 + (((h * 4 + lq) ^ (r & 7)) * 16));
             }
+        if (part) return;
         if constexpr (PHASE == APPLY) {
             unsigned at[FN];
 #pragma unroll
@@ -812,15 +826,15 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
                 }
         }
     };
-    auto multiply = [&](const Fragments& f) {
+    auto multiply = [&](const Fragments& f, int part) {
 #pragma unroll
         for (int n = 0; n < (WIDE ? 3 : 2); ++n)        // hi hi, hi lo, lo hi; or two halves of the step
 #pragma unroll
-            for (int x = 0; x < FM; ++x)
+            for (int x = 0; x < FP; ++x)
 #pragma unroll
                 for (int y = 0; y < FN; ++y)
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        f.c[WIDE ? n >> 1 : n][y], f.r[WIDE ? n & 1 : n][x], acc[x][y], 0, 0, 0);
+                    acc[part * FP + x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        f.c[WIDE ? n >> 1 : n][y], f.r[WIDE ? n & 1 : n][x], acc[part * FP + x][y], 0, 0, 0);
     };
     auto await = [&](int k) {
         if (k + G::kStages - 2 < mine) await_stage<(G::kStages - 2) * kLoads>();
@@ -835,13 +849,16 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
         const bool second = __builtin_amdgcn_readfirstlane(wave) >= kWaves / 2;
         if (second) await(0);
         for (int k = 0; k < steps; ++k) {
-            if (second) turn();
-            else await(k);
-            read(k, f);
-            if (k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
-            if (second) await(k + 1);
-            else turn();
-            multiply(f);
+#pragma unroll
+            for (int part = 0; part < G::kParts; ++part) {
+                if (second || part) turn();
+                else await(k);
+                read(k, part, f);
+                if (!part && k + G::kStages - 1 < steps) stage(k + G::kStages - 1);
+                if (second && part == G::kParts - 1) await(k + 1);
+                else turn();
+                multiply(f, part);
+            }
         }
         if (!second) turn();
     } else if constexpr (PHASE != APPLY) {
@@ -850,14 +867,14 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
         Fragments f0, f1;
         if (G::kStages - 1 < mine) stage(G::kStages - 1);
         await(0);
-        read(0, f0);
+        read(0, 0, f0);
         auto step = [&](int k, const Fragments& now, Fragments& next) {
             if (k + 1 < steps) {
                 await(k + 1);
                 if (k + G::kStages < mine) stage(k + G::kStages);
-                read(k + 1, next);
+                read(k + 1, 0, next);
             }
-            if (G::kGroups == 1 || k < mine) multiply(now);
+            if (G::kGroups == 1 || k < mine) multiply(now, 0);
         };
         for (int k = 0; k < steps; k += 2) {
             step(k, f0, f1);
@@ -868,8 +885,8 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
         for (int k = 0; k < steps; ++k) {
             await(k);
             if (k + G::kStages - 1 < mine) stage(k + G::kStages - 1);
-            read(k, f);
-            if (G::kGroups == 1 || k < mine) multiply(f);
+            read(k, 0, f);
+            if (G::kGroups == 1 || k < mine) multiply(f, 0);
         }
     }
     if constexpr (G::kGroups == 2) {        // the second group's sums to the first
@@ -895,18 +912,22 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
         return;
     }
     float* E = (float*)smem;
-    auto put = [&]() {
-        sides.put(rows, cols);
-        __syncthreads();        // the ring's last stage has been read
-        if (group == 0)
 #pragma unroll
-            for (int x = 0; x < FM; ++x)
+    for (int part = 0; part < G::kParts; ++part) {
+        auto put = [&]() {
+            if (part == 0) sides.put(rows, cols);
+            __syncthreads();    // the ring's last stage has been read, or the rows before these
+            if (group == 0 && wi / kRows == part)
 #pragma unroll
-                for (int y = 0; y < FN; ++y)
-                    *(f32x4*)(E + (wi + x * 16 + l15) * LD + wj + y * 16 + lq * 4) = acc[x][y] * s.inv;
-        __syncthreads();
-    };
-    ns_epilogue<G::kM, G::kN, LD, kThreads, G::kM, PHASE, OUT>(E, rows, cols, q, w, ws, it.b, i0, j0, s, res, put);
+                for (int x = 0; x < FM; ++x)
+#pragma unroll
+                    for (int y = 0; y < FN; ++y)
+                        *(f32x4*)(E + (wi % kRows + x * 16 + l15) * LD + wj + y * 16 + lq * 4) = acc[x][y] * s.inv;
+            __syncthreads();
+        };
+        ns_epilogue<kRows, G::kN, LD, kThreads, G::kM, PHASE, OUT>(E, rows + part * kRows, cols, q, w, ws, it.b,
+                                                                   i0 + part * kRows, j0, s, res, put);
+    }
 }
 
 // Adds the parts of split tiles in the order of the summed index and finishes them, a 64 x 64 piece of
@@ -1348,7 +1369,7 @@ int scale_exp(double v) {
 struct NsLaunch {
     NsTable tab, join;          // `join`: the split entries, counted in tiles
     unsigned blocks = 0, join_tiles = 0;
-    int tile = 0;               // 0 big, 1 mid, 2 small, 3 pair, 4 short
+    int tile = 0;               // 0 big, 1 mid, 2 small, 3 pair, 4 huge, 5 short
     double cost = 0;            // estimate, us
     size_t slab_bytes = 0;
 
@@ -1484,12 +1505,14 @@ struct NsLaunch {
         return l;
     }
     static NsLaunch product(const std::vector<NsProblem>& ps, int phase, bool wide) {
-        double cost[5];
-        NsLaunch l[5] = {tiled<BigTile>(ps, phase, wide, cost[0]), tiled<MidTile>(ps, phase, wide, cost[1]),
-                         tiled<SmallTile>(ps, phase, wide, cost[2]), tiled<PairTile>(ps, phase, wide, cost[3]), {}};
-        if (phase != APPLY) l[4] = tiled<ShortTile>(ps, phase, wide, cost[4]);
+        double cost[6];
+        NsLaunch l[6] = {tiled<BigTile>(ps, phase, wide, cost[0]),   tiled<MidTile>(ps, phase, wide, cost[1]),
+                         tiled<SmallTile>(ps, phase, wide, cost[2]), tiled<PairTile>(ps, phase, wide, cost[3]),
+                         tiled<HugeTile>(ps, phase, wide, cost[4]),  tiled<ShortTile>(ps, phase, wide, cost[5])};
         int best = 0;
-        for (int i = 0; i < (phase == APPLY ? 4 : 5); ++i) {
+        for (int i = 0; i < 6; ++i) {
+            if (i == 4 && (wide || phase != APPLY)) continue;
+            if (i == 5 && phase == APPLY) continue;
             l[i].tile = i;
             if (cost[i] < cost[best]) best = i;
         }
@@ -1729,15 +1752,19 @@ void launch_product(const NsLaunch& l, char* ws, float* slab, const NsStep& s, c
                            dim3(256), 0, stream, l.join, ws, slab, s, r);
 }
 template <typename G, bool WIDE>
+void launch_apply(const NsLaunch& l, NsType type, char* ws, float* slab, const NsStep& s, const NsResult& r,
+                  hipStream_t stream) {
+    if (type == NS_BF16) launch_product<G, WIDE, APPLY, bf16_t>(l, ws, slab, s, r, stream);
+    else if (type == NS_F16) launch_product<G, WIDE, APPLY, f16_t>(l, ws, slab, s, r, stream);
+    else launch_product<G, WIDE, APPLY, float>(l, ws, slab, s, r, stream);
+}
+template <typename G, bool WIDE>
 void launch_phase(const NsLaunch& l, int phase, NsType type, char* ws, float* slab, const NsStep& s,
                   const NsResult& r, hipStream_t stream) {
     if (phase == GRAM) launch_product<G, WIDE, GRAM, float>(l, ws, slab, s, r, stream);
     else if (phase == SQUARE) launch_product<G, WIDE, SQUARE, float>(l, ws, slab, s, r, stream);
-    else if (type == NS_BF16) launch_product<G, WIDE, APPLY, bf16_t>(l, ws, slab, s, r, stream);
-    else if (type == NS_F16) launch_product<G, WIDE, APPLY, f16_t>(l, ws, slab, s, r, stream);
-    else launch_product<G, WIDE, APPLY, float>(l, ws, slab, s, r, stream);
+    else launch_apply<G, WIDE>(l, type, ws, slab, s, r, stream);
 }
-
 void launch_short(const NsLaunch& l, int phase, bool wide, char* ws, const NsStep& s, hipStream_t stream) {
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(l.blocks), dim3(ShortTile::kWaves * 64), 0, stream, l.tab, ws, s);
@@ -1783,6 +1810,7 @@ void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, cons
             else if (l.tile == 1) go(MidTile{});
             else if (l.tile == 2) go(SmallTile{});
             else if (l.tile == 3) go(PairTile{});
+            else if (l.tile == 4) launch_apply<HugeTile, false>(l, type, ws, slab, op->step, r, stream);
             else launch_short(l, op->phase, wide, ws, op->step, stream);
         }
     }
