@@ -65,6 +65,9 @@ class NewtonSchulzPlan {
     template <typename T, bool MUON>
     void launch_solo(const Group& g, const void* x, const void* update, const void* result,
                      hipStream_t stream) const;
+    template <typename T, bool MUON, int ROWS>
+    void launch_solo_rows(const Group& g, const void* x, const void* update, const void* result,
+                     hipStream_t stream) const;
     template <typename Prepare, typename SoloRun>
     void chain(char* ws, NsType type, const Prepare& prepare, const SoloRun& solo, void* out, float* p,
                float lr, float decay, hipStream_t stream) const;

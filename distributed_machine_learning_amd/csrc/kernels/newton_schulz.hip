@@ -19,6 +19,7 @@
 #include <cmath>
 #include <stdexcept>
 #include <string>
+#include <type_traits>
 
 #include "dml_common.h"
 #include "dml_newton_schulz.h"
@@ -1090,30 +1091,40 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
 constexpr int kSoloThreads = 1024, kSoloWaves = kSoloThreads / 64;
 constexpr int kSoloCols = 4096;
 constexpr size_t kSoloLds = 156 * 1024;
-constexpr int kSoloParts = 16;              // partial 16 x 16 tiles of A
-constexpr int kSoloRows = 128;              // largest m: 36 tiles of A's upper triangle, 3 a wave
+constexpr int kSoloRows = 128;              // largest m
+constexpr int kSoloBatch = 8;               // loads of a thread in flight
 
-struct SoloPlanes {                         // a matrix in LDS: hi plane, then lo plane
+// A matrix in LDS: hi plane, then lo plane.  Addresses are a part that is the same for the wave and one
+// of the lane; `lanes` makes the latter anew, for kept over the steps they crowd out the registers.
+struct SoloPlanes {
     uint16_t* hi;
-    int plane, ld;
-    __device__ __forceinline__ float at(int i, int j) const {
-        return f16_value(hi[i * ld + j]) + f16_value(hi[plane + i * ld + j]);
+    int plane, ld, of_rows, of_across, of_four;
+    __device__ __forceinline__ void lanes(int lane) {
+        asm volatile("" : "+v"(lane));
+        of_rows = (lane & 15) * ld + (lane >> 4) * 8;
+        of_across = ((lane >> 4) * 8 + ((lane & 15) >> 2)) * ld + (lane & 3) * 4;
+        of_four = (lane & 15) * ld + (lane >> 4) * 4;
     }
-    __device__ __forceinline__ void put(int i, int j, float v) const {
-        uint16_t h, l;
-        split_f16(v, h, l);
-        hi[i * ld + j] = h;
-        hi[plane + i * ld + j] = l;
+    // 16 x 16 tile from (i, j): row lane % 16, four columns from 4 (lane / 16)
+    __device__ __forceinline__ f32x4 four(int i, int j) const {
+        const uint16_t* at = hi + (i * ld + j + of_four);
+        return __builtin_convertvector(*(const f16x4*)at, f32x4) + __builtin_convertvector(*(const f16x4*)(at + plane), f32x4);
+    }
+    __device__ __forceinline__ void put(int i, int j, f32x4 v) const {
+        uint16_t h[4], l[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) split_f16(v[r], h[r], l[r]);
+        uint16_t* at = hi + (i * ld + j + of_four);
+        *(uint2*)at = *(const uint2*)h;
+        *(uint2*)(at + plane) = *(const uint2*)l;
     }
     // 16 rows from i, 32 columns from k: this lane's eight
     __device__ __forceinline__ f16x8 rows(int i, int k, int lo) const {
-        const int lane = threadIdx.x & 63;
-        return *(const f16x8*)(hi + lo * plane + (i + (lane & 15)) * ld + k + (lane >> 4) * 8);
+        return *(const f16x8*)(hi + (lo * plane + i * ld + k + of_rows));
     }
     // 32 rows from k, 16 columns from j, transposed
     __device__ __forceinline__ f16x8 across(int k, int j, int lo) const {
-        const int lane = threadIdx.x & 63;
-        const uint16_t* at = hi + lo * plane + (k + (lane >> 4) * 8 + ((lane & 15) >> 2)) * ld + j + (lane & 3) * 4;
+        const uint16_t* at = hi + (lo * plane + k * ld + j + of_across);
         const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
         const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * ld));
         const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -1123,18 +1134,30 @@ struct SoloPlanes {                         // a matrix in LDS: hi plane, then l
 __host__ __device__ inline int solo_pad(int v) { return (v + 31) / 32 * 32; }
 __host__ __device__ inline size_t solo_lds(int m, int n) {
     const size_t mp = solo_pad(m), np = solo_pad(n);
-    return 4 * mp * (np + 8) + 4 * mp * (mp + 8) + 8 * mp + kSoloParts * 1024;
+    return 4 * mp * (np + 8) + 4 * mp * (mp + 8) + 8 * mp + kSoloWaves * 1024;
 }
-__device__ __forceinline__ f32x4 mfma_wide(f16x8 ah, f16x8 al, f16x8 bh, f16x8 bl, f32x4 acc) {
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bh, acc, 0, 0, 0);
-    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, bl, acc, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(al, bh, acc, 0, 0, 0);
-}
-// Tile t of the upper triangle of 16 x 16 tiles, column by column.
-__device__ __forceinline__ void solo_tile(int t, int& ti, int& tj) {
-    tj = 0;
-    while ((tj + 1) * (tj + 2) / 2 <= t) ++tj;
-    ti = t - tj * (tj + 1) / 2;
+// A 16 x 16 tile of a wide product.  The columns' operand comes first: a lane ends with columns
+// 4 (lane / 16) .. + 3 of row lane % 16.  Two sums, for the chain of one is all latency.
+struct SoloSum {
+    f32x4 high = {0.f, 0.f, 0.f, 0.f}, low = {0.f, 0.f, 0.f, 0.f};
+    __device__ __forceinline__ void add(f16x8 ch, f16x8 cl, f16x8 rh, f16x8 rl) {
+        high = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, rh, high, 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_16x16x32_f16(ch, rl, low, 0, 0, 0);
+        low = __builtin_amdgcn_mfma_f32_16x16x32_f16(cl, rh, low, 0, 0, 0);
+    }
+    // rows i, columns j of X X^T over 32-column steps from .. to
+    __device__ __forceinline__ void gram(const SoloPlanes& x, int i, int j, int from, int to) {
+#pragma unroll 2
+        for (int k = from * 32; k < to * 32; k += 32)
+            add(x.rows(j, k, 0), x.rows(j, k, 1), x.rows(i, k, 0), x.rows(i, k, 1));
+    }
+    __device__ __forceinline__ f32x4 sum() const { return high + low; }
+};
+
+// A power of two near the square root of v, so that v is the product of two floats of modest size.
+__device__ __forceinline__ float solo_power(double v) {
+    const int e = v > 0.0 && v < 1e300 ? ilogb(v) / 2 : 0;
+    return ldexpf(1.f, e);
 }
 
 struct SoloSteps {
@@ -1144,7 +1167,9 @@ struct SoloSteps {
 };
 static_assert(sizeof(NsTable) + sizeof(SoloSteps) <= 4000, "kernel arguments");
 
-template <typename T, bool MUON>
+// Most of a small matrix's time is instructions that are fetched for the first time, so each piece of code
+// is there once: one loop for both passes over the matrix, one tile of A to a wave where ROWS is 64.
+template <typename T, bool MUON, int ROWS>
 __global__ __launch_bounds__(kSoloThreads) void ns_solo_kernel(NsTable tab, const T* __restrict__ x, NsUpdate u,
                                                                double eps, SoloSteps st, NsResult res) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1162,97 +1187,170 @@ __global__ __launch_bounds__(kSoloThreads) void ns_solo_kernel(NsTable tab, cons
     float* d = (float*)(sq.hi + 2 * sq.plane);      // diagonal of A
     float* e = d + mp;                              // diagonal of P
     float* parts = e + mp;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, l15 = lane & 15, lq = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, l15 = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);     // tiles by scalar arithmetic
 
-    // norm (and momentum)
+    // The norm, and in the update the momentum, then the planes.  A lane takes four consecutive elements of
+    // a row where all of them allow a vector load, else one; a wave takes 64 such groups of a row or, where
+    // rows are shorter, several rows, so that no element needs a division.
     const long long src = q.src + b * q.stride;
-    const int count = q.rows * q.cols;
-    double sum = 0.0;
-    for (int k = tid; k < count; k += kSoloThreads) {
-        const long long at = src + (long long)(k / q.cols) * q.ld + k % q.cols;
-        float v;
-        if constexpr (MUON) {
-            const float g = u.g[at] * u.grad_scale;
-            const float m = u.mu * u.m[at] + g;
-            u.m[at] = m;
-            v = u.nesterov ? g + u.mu * m : m;
-        } else {
-            v = ns_elem(x[at]);
-        }
-        sum += (double)v * (double)v;
-    }
-    double* sums = (double*)parts;
+    for (int k = tid; k < (y.plane + sq.plane) / 4; k += kSoloThreads) ((uint4*)y.hi)[k] = uint4{0, 0, 0, 0};
+    const int sr = q.trans ? 1 : y.ld, sc = q.trans ? y.ld : 1;
+    auto read = [&](auto vector) {
+        constexpr int V = decltype(vector)::value, kBatch = V == 4 ? 4 : 8;     // loads in flight
+        const int groups = q.cols / V;
+        const int shift = groups >= 64 ? 6 : 32 - __clz(groups - 1);        // (one group: __clz(0) is 32)
+        const int high = 64 >> shift, chunks = (groups + 63) >> 6;
+        const int units = (q.rows + high - 1) / high * chunks;
+        const int turns = (units - wave + kSoloWaves - 1) / kSoloWaves;     // of this wave
+        const int lr = lane >> shift, lc = (lane & ((1 << shift) - 1)) * V;
+        const int down = kSoloWaves / chunks, right = kSoloWaves % chunks;
+        const long long lane_at = (long long)lr * q.ld + lc;
+        struct Place { int row, col; };
+        auto inside = [&](const Place& p) { return p.row + lr < q.rows && p.col + lc < q.cols; };
+        auto advance = [&](Place& p) {
+            p.row += down * high;
+            p.col += right * 64 * V;
+            if (p.col >= chunks * 64 * V) {
+                p.col -= chunks * 64 * V;
+                p.row += high;
+            }
+        };
+        auto load = [&](const auto* from, float (&v)[V]) {
+            typedef typename std::remove_cv<typename std::remove_pointer<decltype(from)>::type>::type E;
+            struct alignas(V * sizeof(E)) Group { E e[V]; };
+            const Group w = *(const Group*)from;
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    if (lane == 0) sums[wave] = sum;
-    __syncthreads();
-    sum = 0.0;
-    for (int k = 0; k < kSoloWaves; ++k) sum += sums[k];
-    const double inv = (double)st.sy / (sqrt(sum) + eps);
-    for (int k = tid; k < y.plane; k += kSoloThreads) ((uint32_t*)y.hi)[k] = 0;
-    __syncthreads();
-    for (int k = tid; k < count; k += kSoloThreads) {
-        const int r = k / q.cols, c = k % q.cols;
-        const long long at = src + (long long)r * q.ld + c;
-        float v;
-        if constexpr (MUON) {
-            const float m = u.m[at];        // this thread's own, written above
-            v = u.nesterov ? u.g[at] * u.grad_scale + u.mu * m : m;
-        } else {
-            v = ns_elem(x[at]);
+            for (int j = 0; j < V; ++j) v[j] = ns_elem(w.e[j]);
+        };
+        double sum = 0.0;
+        float power = 0.f, scale = 0.f;
+#pragma unroll 1
+        for (int pass = 0; pass < 2; ++pass) {
+            Place p{wave / chunks * high, wave % chunks * 64 * V};
+#pragma unroll 1
+            for (int n0 = 0; n0 < turns; n0 += kBatch) {
+                float v[kBatch][V], m[kBatch][V];
+                Place at = p;
+#pragma unroll
+                for (int n = 0; n < kBatch; ++n) {
+                    const long long from = src + (long long)at.row * q.ld + at.col;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v[n][j] = m[n][j] = 0.f;
+                    if (inside(at)) {
+                        if constexpr (MUON) {
+                            load(u.g + from + lane_at, v[n]);
+                            load((const float*)u.m + from + lane_at, m[n]);
+                        } else {
+                            load(x + from + lane_at, v[n]);
+                        }
+                    }
+                    advance(at);
+                }
+#pragma unroll
+                for (int n = 0; n < kBatch; ++n) {
+                    const bool in = inside(p);
+                    if constexpr (MUON) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) {
+                            const float g = v[n][j] * u.grad_scale;
+                            if (pass == 0) m[n][j] = u.mu * m[n][j] + g;
+                            v[n][j] = u.nesterov ? g + u.mu * m[n][j] : m[n][j];
+                        }
+                        if (pass == 0 && in) {
+                            struct alignas(V * 4) Group { float e[V]; } w;
+#pragma unroll
+                            for (int j = 0; j < V; ++j) w.e[j] = m[n][j];
+                            *(Group*)(u.m + (src + (long long)p.row * q.ld + p.col) + lane_at) = w;
+                        }
+                    }
+                    if (pass == 0) {
+#pragma unroll
+                        for (int j = 0; j < V; ++j) sum += (double)v[n][j] * (double)v[n][j];
+                    } else if (in) {
+                        uint16_t h[V], l[V];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) split_f16(v[n][j] * power * scale, h[j], l[j]);
+                        uint16_t* to = y.hi + (p.row * sr + p.col * sc + lr * sr + lc * sc);
+                        if (V == 4 && !q.trans) {
+                            *(uint2*)to = *(const uint2*)h;
+                            *(uint2*)(to + y.plane) = *(const uint2*)l;
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < V; ++j) {
+                                to[j * sc] = h[j];
+                                to[j * sc + y.plane] = l[j];
+                            }
+                        }
+                    }
+                    advance(p);
+                }
+            }
+            if (pass == 0) {
+                double* sums = (double*)parts;
+#pragma unroll
+                for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+                if (lane == 0) sums[wave] = sum;
+                __syncthreads();
+                sum = sums[0];
+#pragma unroll
+                for (int k = 1; k < kSoloWaves; ++k) sum += sums[k];
+                // 1 / norm may be out of fp32's range: it is applied as two factors, neither of which is
+                const double inv = (double)st.sy / (sqrt(sum) + eps);
+                power = solo_power(inv);
+                scale = (float)(inv / (double)power);
+            }
         }
-        v = (float)((double)v * inv);
-        if (q.trans) y.put(c, r, v);
-        else y.put(r, c, v);
-    }
+    };
+    const int esize = MUON ? 4 : (int)sizeof(T);
+    const size_t at0 = (MUON ? (size_t)u.g | (size_t)u.m : (size_t)x) + (size_t)src * esize;
+    if (q.cols % 4 == 0 && q.ld % 4 == 0 && at0 % (4 * esize) == 0) read(std::integral_constant<int, 4>{});
+    else read(std::integral_constant<int, 1>{});
     __syncthreads();
 
-    const int tm = mp / 16, tiles = tm * (tm + 1) / 2, ksteps = np / 32;
-    const int cuts = tiles >= kSoloParts ? 1 : (kSoloParts / tiles < ksteps ? kSoloParts / tiles : ksteps);
+    // All tiles of the symmetric matrices: no more rounds of the 16 waves than their upper triangle
+    // takes (one more from 81 rows on), and no mirrored writes.  Rows are padded to 16 here, sums over
+    // rows to 32 by zeros that nothing overwrites.
+    constexpr int kOwn = (ROWS / 16) * (ROWS / 16) / kSoloWaves;        // tiles of a wave
+    const int tm = (q.m + 15) / 16, tiles = tm * tm, ksteps = np / 32;
+    const int cuts = tiles >= kSoloWaves ? 1 : min(kSoloWaves / tiles, ksteps);
     const float inv_a = 1.f / (st.sy * st.sy), inv_p = 1.f / (st.sa * st.sa), inv_y = 1.f / (st.sp * st.sy);
-    constexpr int kOwn = (kSoloRows / 16 * (kSoloRows / 16 + 1) / 2 + kSoloWaves - 1) / kSoloWaves;
+    const float un_a = 1.f / st.sa, un_y = 1.f / st.sy;
     for (int step = 0; step < st.steps; ++step) {
+        y.lanes(lane);
+        sq.lanes(lane);
         const float ka = st.k[3 * step], kb = st.k[3 * step + 1], kc = st.k[3 * step + 2];
         f32x4 acc[kOwn];
-        // A = Y Y^T: a wave takes tiles of the upper triangle or, where they are few, parts of their sums
-        if (cuts > 1) {
-            if (wave < tiles * cuts) {
-                int ti, tj;
-                solo_tile(wave / cuts, ti, tj);
-                const int cut = wave % cuts;
-                f32x4 a = {0.f, 0.f, 0.f, 0.f};
-                for (int k = ksteps * cut / cuts; k < ksteps * (cut + 1) / cuts; ++k)
-                    a = mfma_wide(y.rows(ti * 16, k * 32, 0), y.rows(ti * 16, k * 32, 1), y.rows(tj * 16, k * 32, 0),
-                                  y.rows(tj * 16, k * 32, 1), a);
-                *(f32x4*)(parts + (wave * 64 + lane) * 4) = a;
-            }
-            __syncthreads();
-        }
+        // A = Y Y^T: a wave takes whole tiles or, where they are few, a part of one's sum
 #pragma unroll
         for (int n = 0; n < kOwn; ++n) {
-            const int t = wave + n * kSoloWaves;
-            if (t >= tiles) break;
-            int ti, tj;
-            solo_tile(t, ti, tj);
-            f32x4 a = {0.f, 0.f, 0.f, 0.f};
+            int t = cuts > 1 ? wave / cuts : wave + n * kSoloWaves;
+            if (cuts == 1 ? t >= tiles : n > 0) break;
+            const int cut = cuts > 1 ? wave % cuts : 0;
+            f32x4 z = {0.f, 0.f, 0.f, 0.f};
+            if (t < tiles) {
+                SoloSum a;
+                a.gram(y, t / tm * 16, t % tm * 16, ksteps * cut / cuts, ksteps * (cut + 1) / cuts);
+                z = a.sum();
+            }
             if (cuts > 1) {
-                for (int k = 0; k < cuts; ++k) a += *(const f32x4*)(parts + ((t * cuts + k) * 64 + lane) * 4);
-            } else {
-                for (int k = 0; k < ksteps; ++k)
-                    a = mfma_wide(y.rows(ti * 16, k * 32, 0), y.rows(ti * 16, k * 32, 1), y.rows(tj * 16, k * 32, 0),
-                                  y.rows(tj * 16, k * 32, 1), a);
+                *(f32x4*)(parts + (wave * 64 + lane) * 4) = z;
+                __syncthreads();
+                t = wave;
+                if (t >= tiles) break;
+                z = *(const f32x4*)(parts + (t * cuts * 64 + lane) * 4);
+#pragma unroll 4
+                for (int k = 1; k < cuts; ++k) z += *(const f32x4*)(parts + ((t * cuts + k) * 64 + lane) * 4);
             }
+            const int ti = t / tm * 16, tj = t % tm * 16, i = ti + l15, j = tj + lq * 4;
+            z *= inv_a;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = ti * 16 + lq * 4 + r, j = tj * 16 + l15;
-                float z = a[r] * inv_a;
-                if (i == j) {
-                    d[i] = z;
-                    z = 0.f;
+            for (int r = 0; r < 4; ++r)
+                if (i == j + r) {
+                    d[i] = z[r];
+                    z[r] = 0.f;
                 }
-                sq.put(i, j, z * st.sa);
-                if (ti != tj) sq.put(j, i, z * st.sa);
-            }
+            sq.put(ti, tj, z * st.sa);
         }
         __syncthreads();
         // P = b A + c A A in place of A, its diagonal with the a
@@ -1260,68 +1358,82 @@ __global__ __launch_bounds__(kSoloThreads) void ns_solo_kernel(NsTable tab, cons
         for (int n = 0; n < kOwn; ++n) {
             const int t = wave + n * kSoloWaves;
             if (t >= tiles) break;
-            int ti, tj;
-            solo_tile(t, ti, tj);
-            f32x4 a = {0.f, 0.f, 0.f, 0.f};
-            for (int k = 0; k < mp / 32; ++k)
-                a = mfma_wide(sq.rows(ti * 16, k * 32, 0), sq.rows(ti * 16, k * 32, 1), sq.rows(tj * 16, k * 32, 0),
-                              sq.rows(tj * 16, k * 32, 1), a);
+            const int ti = t / tm * 16, tj = t % tm * 16, i = ti + l15, j = tj + lq * 4;
+            const f32x4 o = sq.four(ti, tj) * un_a, dj = *(const f32x4*)(d + j);
+            const float di = d[i];
+            SoloSum a;
+            a.gram(sq, ti, tj, 0, mp / 32);
+            const f32x4 z = a.sum() * inv_p;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = ti * 16 + lq * 4 + r, j = tj * 16 + l15;
-                const float di = d[i], dj = d[j], o = sq.at(i, j) / st.sa, z = a[r] * inv_p;
-                acc[n][r] = i == j ? kc * (z + di * di) + (kb * di + ka) : kc * (z + (di + dj) * o) + kb * o;
-            }
+            for (int r = 0; r < 4; ++r)
+                acc[n][r] = i == j + r ? kc * (z[r] + di * di) + (kb * di + ka)
+                                       : kc * (z[r] + (di + dj[r]) * o[r]) + kb * o[r];
         }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < kOwn; ++n) {
             const int t = wave + n * kSoloWaves;
             if (t >= tiles) break;
-            int ti, tj;
-            solo_tile(t, ti, tj);
+            const int ti = t / tm * 16, tj = t % tm * 16, i = ti + l15, j = tj + lq * 4;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int i = ti * 16 + lq * 4 + r, j = tj * 16 + l15;
-                float z = acc[n][r];
-                if (i == j) {
-                    e[i] = z;
-                    z = 0.f;
+            for (int r = 0; r < 4; ++r)
+                if (i == j + r) {
+                    e[i] = acc[n][r];
+                    acc[n][r] = 0.f;
                 }
-                sq.put(i, j, z * st.sp);
-                if (ti != tj) sq.put(j, i, z * st.sp);
-            }
+            sq.put(ti, tj, acc[n] * st.sp);
         }
         __syncthreads();
         // Y <- P Y: a wave takes columns, whose old values it has read before it writes the new ones
         const bool last = step == st.steps - 1;
+#pragma unroll 1
         for (int tj = wave; tj < np / 16; tj += kSoloWaves) {
-            f16x8 ch[kSoloRows / 32], cl[kSoloRows / 32];
+            f16x8 ch[ROWS / 32], cl[ROWS / 32];
 #pragma unroll
-            for (int k = 0; k < kSoloRows / 32; ++k)
+            for (int k = 0; k < ROWS / 32; ++k)
                 if (k < mp / 32) {
                     ch[k] = y.across(k * 32, tj * 16, 0);
                     cl[k] = y.across(k * 32, tj * 16, 1);
                 }
+#pragma unroll 1
             for (int ti = 0; ti < tm; ++ti) {
-                f32x4 a = {0.f, 0.f, 0.f, 0.f};
+                const int i = ti * 16 + l15, j = tj * 16 + lq * 4;
+                const f32x4 old = y.four(ti * 16, tj * 16) * un_y;
+                const float ei = e[i];
+                SoloSum a;
 #pragma unroll
-                for (int k = 0; k < kSoloRows / 32; ++k)
-                    if (k < mp / 32) a = mfma_wide(sq.rows(ti * 16, k * 32, 0), sq.rows(ti * 16, k * 32, 1), ch[k], cl[k], a);
+                for (int k = 0; k < ROWS / 32; ++k)
+                    if (k < mp / 32) a.add(ch[k], cl[k], sq.rows(ti * 16, k * 32, 0), sq.rows(ti * 16, k * 32, 1));
+                const f32x4 z = old * ei + a.sum() * inv_y;
+                if (!last) {
+                    y.put(ti * 16, tj * 16, z * st.sy);
+                    continue;
+                }
+                if (!q.trans && i < q.m && j + 4 <= q.n) {
+                    if constexpr (MUON) {
+                        float* at = res.p + src + (long long)i * q.ld + j;
+                        if (((uintptr_t)at & 15) == 0) {
+                            *(f32x4*)at = res.decay * *(f32x4*)at - res.lr * q.lr * z;
+                            continue;
+                        }
+                    } else {
+                        T* at = (T*)res.out + q.out + b * q.out_stride + (long long)i * q.out_ld + j;
+                        struct alignas(4 * sizeof(T)) Four { T e[4]; };
+                        if (((uintptr_t)at & (sizeof(Four) - 1)) == 0) {
+                            *(Four*)at = Four{{(T)z[0], (T)z[1], (T)z[2], (T)z[3]}};
+                            continue;
+                        }
+                    }
+                }
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int i = ti * 16 + lq * 4 + r, j = tj * 16 + l15;
-                    const float z = e[i] * (y.at(i, j) / st.sy) + a[r] * inv_y;
-                    if (!last) {
-                        y.put(i, j, z * st.sy);
-                    } else if (i < q.m && j < q.n) {
-                        const long long row = q.trans ? j : i, col = q.trans ? i : j;
-                        if (MUON) {
-                            float* at = res.p + src + row * q.ld + col;
-                            *at = res.decay * *at - res.lr * q.lr * z;
-                        } else {
-                            ((T*)res.out)[q.out + b * q.out_stride + row * q.out_ld + col] = (T)z;
-                        }
+                    if (i >= q.m || j + r >= q.n) continue;
+                    const long long row = q.trans ? j + r : i, col = q.trans ? i : j + r;
+                    if (MUON) {
+                        float* at = res.p + src + row * q.ld + col;
+                        *at = res.decay * *at - res.lr * q.lr * z[r];
+                    } else {
+                        ((T*)res.out)[q.out + b * q.out_stride + row * q.out_ld + col] = (T)z[r];
                     }
                 }
             }
@@ -1539,6 +1651,7 @@ struct NewtonSchulzPlan::Group {
 struct NewtonSchulzPlan::Solo {
     SoloSteps steps{};
     size_t lds = 0;
+    int rows = 0;               // the most of a matrix's smaller side
 };
 struct NewtonSchulzPlan::Op {
     int phase;
@@ -1613,6 +1726,8 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
     if (solo) {
         solo_ = std::make_shared<Solo>();
         solo_->lds = lds;
+        for (const auto& ps : sets)
+            for (const NsProblem& p : ps) solo_->rows = std::max(solo_->rows, p.m);
         SoloSteps& st = solo_->steps;
         st.steps = steps;
         double amax = 1e-3;
@@ -1775,16 +1890,23 @@ void launch_short(const NsLaunch& l, int phase, bool wide, char* ws, const NsSte
 
 }  // namespace
 
+template <typename T, bool MUON, int ROWS>
+void NewtonSchulzPlan::launch_solo_rows(const Group& g, const void* x, const void* update, const void* result,
+                                   hipStream_t stream) const {
+    // (more than the default 64 KB of LDS has to be allowed once per device)
+    const void* f = (const void*)ns_solo_kernel<T, MUON, ROWS>;
+    if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kSoloLds) != hipSuccess)
+        throw std::runtime_error("newton_schulz: hipFuncSetAttribute");
+    hipLaunchKernelGGL((ns_solo_kernel<T, MUON, ROWS>), dim3(g.solo.blocks), dim3(kSoloThreads), solo_->lds, stream,
+                       g.solo.tab, (const T*)x, *(const NsUpdate*)update, eps_, solo_->steps,
+                       *(const NsResult*)result);
+}
+
 template <typename T, bool MUON>
 void NewtonSchulzPlan::launch_solo(const Group& g, const void* x, const void* update, const void* result,
                                    hipStream_t stream) const {
-    // (more than the default 64 KB of LDS has to be allowed once per device)
-    const void* f = (const void*)ns_solo_kernel<T, MUON>;
-    if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kSoloLds) != hipSuccess)
-        throw std::runtime_error("newton_schulz: hipFuncSetAttribute");
-    hipLaunchKernelGGL((ns_solo_kernel<T, MUON>), dim3(g.solo.blocks), dim3(kSoloThreads), solo_->lds, stream,
-                       g.solo.tab, (const T*)x, *(const NsUpdate*)update, eps_, solo_->steps,
-                       *(const NsResult*)result);
+    if (solo_->rows <= 64) launch_solo_rows<T, MUON, 64>(g, x, update, result, stream);
+    else launch_solo_rows<T, MUON, kSoloRows>(g, x, update, result, stream);
 }
 
 template <typename Prepare, typename SoloRun>
