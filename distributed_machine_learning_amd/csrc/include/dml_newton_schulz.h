@@ -75,7 +75,7 @@ class NewtonSchulzPlan {
     std::vector<NsSegment> segs_;
     std::vector<float> coef_;
     double eps_;
-    bool wide_, squares_wide_ = false;
+    bool wide_, squares_wide_ = false, fused_ = false;
     int x_exp_;                      // Y's planes hold value * 2^exp
     std::vector<std::shared_ptr<Op>> ops_;
     std::shared_ptr<Solo> solo_;

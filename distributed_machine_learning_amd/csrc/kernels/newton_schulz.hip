@@ -1086,8 +1086,10 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
 
 // ------------------------------------------------------------------ one block per matrix
 // Where Y and one m x m matrix fit a CU's LDS, a block runs the whole chain of a matrix by itself:
-// one launch instead of 17 or more, no memory traffic but the matrix itself.  Rows are padded to
+// one launch instead of 12 or more, no memory traffic but the matrix itself.  Rows are padded to
 // multiples of 32, pitches by 8 elements so that the 16 rows of a fragment meet different banks.
+// Latency of barriers and dependent LDS reads bounds it: 64 x 27 takes 21 us, 10 x 512 25, 64 x 448 57
+// (grouped launches: 64 x 520 82), 32 x 1088 51 (32 x 1200 89), 128 x 128 86 (128 x 192 85).
 constexpr int kSoloThreads = 1024, kSoloWaves = kSoloThreads / 64;
 constexpr int kSoloCols = 4096;
 constexpr size_t kSoloLds = 156 * 1024;
@@ -1442,6 +1444,110 @@ __global__ __launch_bounds__(kSoloThreads) void ns_solo_kernel(NsTable tab, cons
     }
 }
 
+// ------------------------------------------------------------------ A A and B Y in one launch
+// Where A is small, a block that makes a 64 x 64 tile of the next Y first makes the 64 rows of P that it
+// needs: 64 m^2 multiplications next to the tile's 64^2 m, and one launch less per step.  A block fills
+// its CU's LDS, so this pays for one round of blocks (96 x 320: 80 us against 92, 128 x 8192: 157 against
+// 172) and not for several (24 of 128 x 1024, 768 blocks: 198 against 151).
+constexpr int kFusedRows = 128;             // largest padded m
+constexpr double kFusedUs = 8;              // of a block; one to a CU
+template <typename OUT>
+__global__ __launch_bounds__(512) void ns_fused_kernel(NsTable tab, char* ws, NsStep sq, NsStep s, NsResult res) {
+    constexpr int R = kFusedRows, LD = 68;
+    __shared__ __attribute__((aligned(16))) uint16_t amem[2 * R * (R + 8)], pmem[2 * 64 * (R + 8)], ymem[2 * R * 72];
+    __shared__ __attribute__((aligned(16))) float d[R], e[64];
+    const NsItem it = item_of<SmallTile, APPLY>(tab, blockIdx.x, gridDim.x);
+    const NsProblem& q = tab.p[it.problem];
+    const NsPlanes w = ns_planes(q, ws, it.b, s.buffer);
+    const int t = threadIdx.x, lane = t & 63, l15 = lane & 15, lq = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int i0 = it.ti * 64, j0 = it.tj * 64, mp = q.mp;
+    SoloPlanes a, p, y;
+    a.hi = amem; a.ld = mp + 8; a.plane = mp * a.ld;
+    p.hi = pmem; p.ld = mp + 8; p.plane = 64 * p.ld;
+    y.hi = ymem; y.ld = 72; y.plane = mp * 72;
+    a.lanes(lane);
+    p.lanes(lane);
+    y.lanes(lane);
+
+    // A and a column of Y's tiles to LDS, all loads in flight at once
+    constexpr int kA = R * R / 4 / 512, kY = R * 16 / 512;
+    const uint16_t* from = w.square(sq.x);
+    typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
+    const int shift = mp == 64 ? 3 : 4;         // 8 or 16 pieces of 16 bytes in a row of A
+    u32x4 va[kA], vy[kY];
+#pragma unroll
+    for (int n = 0; n < kA; ++n) {
+        const int at = t + n * 512, r = at >> shift, c = (at & ((1 << shift) - 1)) * 8;
+        const int row = r < 2 * mp ? r : 0;     // rows of the hi, then of the lo plane
+        va[n] = *(const u32x4*)(from + (row >= mp ? w.aplane : 0) + (row >= mp ? row - mp : row) * w.ald + c);
+    }
+#pragma unroll
+    for (int n = 0; n < kY; ++n) {
+        const int at = t + n * 512, r = at >> 3, c = (at & 7) * 8, row = r < 2 * mp ? r : 0;
+        vy[n] = *(const u32x4*)(w.y + (row >= mp ? w.yplane : 0) + (size_t)(row >= mp ? row - mp : row) * w.yld + j0 + c);
+    }
+    const float dt = w.diagonal(sq.x)[t < mp ? t : 0];
+#pragma unroll
+    for (int n = 0; n < kA; ++n) {
+        const int at = t + n * 512, row = at >> shift, c = (at & ((1 << shift) - 1)) * 8;
+        if (row < 2 * mp) *(u32x4*)(amem + row * a.ld + c) = va[n];
+    }
+#pragma unroll
+    for (int n = 0; n < kY; ++n) {
+        const int at = t + n * 512, row = at >> 3, c = (at & 7) * 8;
+        if (row < 2 * mp) *(u32x4*)(ymem + row * 72 + c) = vy[n];
+    }
+    if (t < mp) d[t] = dt;
+    __syncthreads();
+
+    // rows i0 .. i0 + 63 of P: a wave takes 32 of them and a quarter of the columns
+    const int wr = (wave >> 2) * 32, quarter = wave & 3;
+    for (int c = quarter * (mp / 4); c < (quarter + 1) * (mp / 4); c += 16) {
+        SoloSum sum[2];
+#pragma unroll 2
+        for (int k = 0; k < mp; k += 32) {
+            const f16x8 ch = a.rows(c, k, 0), cl = a.rows(c, k, 1);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) sum[x].add(ch, cl, a.rows(i0 + wr + x * 16, k, 0), a.rows(i0 + wr + x * 16, k, 1));
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int i = i0 + wr + x * 16 + l15, j = c + lq * 4;
+            const f32x4 o = a.four(i0 + wr + x * 16, c) * sq.iw, dj = *(const f32x4*)(d + j);
+            const float di = d[i];
+            f32x4 z = sum[x].sum() * sq.inv;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                z[r] = i == j + r ? sq.k1 * (z[r] + di * di) + (sq.k2 * di + sq.k0)
+                                  : sq.k1 * (z[r] + (di + dj[r]) * o[r]) + sq.k2 * o[r];
+                if (i == j + r) {
+                    e[i - i0] = z[r];
+                    z[r] = 0.f;
+                }
+            }
+            p.put(wr + x * 16, c, z * sq.sz);
+        }
+    }
+    __syncthreads();
+    SoloSum sum[2];
+    const int wc = quarter * 16;
+#pragma unroll 2
+    for (int k = 0; k < mp; k += 32) {
+        const f16x8 ch = y.across(k, wc, 0), cl = y.across(k, wc, 1);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) sum[x].add(ch, cl, p.rows(wr + x * 16, k, 0), p.rows(wr + x * 16, k, 1));
+    }
+    float* E = (float*)amem;        // A has been read before the last barrier
+    auto put = [&]() {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            *(f32x4*)(E + (wr + x * 16 + l15) * LD + wc + lq * 4) = sum[x].sum() * s.inv;
+        __syncthreads();
+    };
+    ns_epilogue<64, 64, LD, 512, 64, APPLY, OUT>(E, e, nullptr, q, w, ws, it.b, i0, j0, s, res, put);
+}
+
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
 // Largest |a x + b x^3 + c x^5| over [0, r].
@@ -1616,6 +1722,17 @@ struct NsLaunch {
         l.slab_bytes = (size_t)slab * G::kM * G::kN * sizeof(float);
         return l;
     }
+    // A A and B Y in one launch, where every A fits it
+    static NsLaunch fused(const std::vector<NsProblem>& ps) {
+        NsLaunch l{};
+        for (const NsProblem& p : ps)
+            if (p.mp > kFusedRows) return l;
+        double cost;
+        l = tiled<SmallTile>(ps, APPLY, true, cost);
+        if (l.join_tiles) return NsLaunch{};
+        l.cost = kFusedUs * ((l.blocks + kCus - 1) / kCus) + 2.5;
+        return l;
+    }
     static NsLaunch product(const std::vector<NsProblem>& ps, int phase, bool wide) {
         double cost[6];
         NsLaunch l[6] = {tiled<BigTile>(ps, phase, wide, cost[0]),   tiled<MidTile>(ps, phase, wide, cost[1]),
@@ -1636,11 +1753,11 @@ struct NsLaunch {
 }  // namespace
 
 struct NewtonSchulzPlan::Group {
-    NsLaunch norm, load, product[3], wide_square, solo;
+    NsLaunch norm, load, product[3], wide_square, fused, solo;
     // The workspace of the problem whose partial sums start at `part`, in every table.
     void place(int part, long long ws, long long stride) {
         for (NsTable* t : {&norm.tab, &load.tab, &product[0].tab, &product[1].tab, &product[2].tab,
-                           &product[0].join, &product[1].join, &product[2].join})
+                           &product[0].join, &product[1].join, &product[2].join, &fused.tab})
             for (int i = 0; i < t->count; ++i)
                 if (t->p[i].part == part) {
                     t->p[i].ws = ws;
@@ -1764,7 +1881,8 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         chains.push_back(n);
         k += n;
     }
-    double single_us = 0, chain_us = 0;
+    double single_us = 0, chain_us = 0, fused_us = 0;
+    bool can_fuse = wide_;
     for (const auto& ps : sets) {
         groups_.push_back(std::make_shared<Group>());
         Group& g = *groups_.back();
@@ -1775,8 +1893,13 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         const double ends = g.product[GRAM].cost + g.product[APPLY].cost;
         single_us += steps * (ends + g.product[SQUARE].cost);
         for (int n : chains) chain_us += ends + (4 * n - 3) * g.wide_square.cost;
+        g.fused = NsLaunch::fused(ps);
+        can_fuse = can_fuse && g.fused.blocks;
+        fused_us += steps * (g.product[GRAM].cost + g.fused.cost);
     }
-    const bool chained = (int)chains.size() < steps && chain_us < 0.95 * single_us;
+    fused_ = can_fuse && fused_us < single_us;
+    const bool chained = (int)chains.size() < steps && chain_us < 0.95 * (fused_ ? fused_us : single_us);
+    if (chained) fused_ = false;
     if (!chained) chains.assign(steps, 1);
     size_t slab = 0;
     for (const auto& g : groups_) {
@@ -1880,6 +2003,13 @@ void launch_phase(const NsLaunch& l, int phase, NsType type, char* ws, float* sl
     else if (phase == SQUARE) launch_product<G, WIDE, SQUARE, float>(l, ws, slab, s, r, stream);
     else launch_apply<G, WIDE>(l, type, ws, slab, s, r, stream);
 }
+void launch_fused(const NsLaunch& l, NsType type, char* ws, const NsStep& square, const NsStep& s, const NsResult& r,
+                  hipStream_t stream) {
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(l.blocks), dim3(512), 0, stream, l.tab, ws, square, s, r); };
+    if (type == NS_BF16) go(ns_fused_kernel<bf16_t>);
+    else if (type == NS_F16) go(ns_fused_kernel<f16_t>);
+    else go(ns_fused_kernel<float>);
+}
 void launch_short(const NsLaunch& l, int phase, bool wide, char* ws, const NsStep& s, hipStream_t stream) {
     auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(l.blocks), dim3(ShortTile::kWaves * 64), 0, stream, l.tab, ws, s);
@@ -1920,7 +2050,13 @@ void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, cons
             continue;
         }
         prepare(*g, (double*)(ws + partials_), std::ldexp(1.f, x_exp_));
+        const NsStep* before = nullptr;
         for (const auto& op : ops_) {
+            if (fused_ && op->phase != GRAM) {
+                if (op->phase == APPLY) launch_fused(g->fused, type, ws, *before, op->step, r, stream);
+                before = &op->step;
+                continue;
+            }
             const NsLaunch& l = g->product[op->phase];
             const bool wide = op->phase == SQUARE ? squares_wide_ : wide_;
             auto go = [&](auto tile) {
