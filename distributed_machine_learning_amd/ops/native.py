@@ -584,6 +584,7 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     wide = _ns_wide(precision, x.dtype, min(x.shape[-2:]))
     if x.numel() == 0:
         return torch.empty_like(x)
+    x = x.resolve_neg()
     layout = _ns_layout(x)
     if layout is None:
         x = x.contiguous()
@@ -642,6 +643,9 @@ def muon_step_(plan: MuonPlan, p: torch.Tensor, g: torch.Tensor, m: torch.Tensor
             raise ValueError(f"muon_step_: {n} is on {t.device}, p on {p.device}")
         if t.numel() != p.numel() or t.numel() < plan.elems:
             raise ValueError(f"muon_step_: {n} has {t.numel()} elements, p {p.numel()}, the plan needs {plan.elems}")
+    first, second, third = sorted(t.data_ptr() for t in (p, g, m))
+    if p.numel() and min(second - first, third - second) < 4 * p.numel():
+        raise ValueError("muon_step_: p, g and m must not overlap")
     if workspace is None:
         workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=p.device)
     else:

@@ -10,8 +10,8 @@ def triples(steps, coefficients):
     return [c] * steps if len(c) == 3 and not hasattr(c[0], "__len__") else c
 
 
-def exact(x, steps=5, coefficients=NS, eps=1e-7):
-    y = x.detach().cpu().double()
+def exact(x, steps=5, coefficients=NS, eps=1e-7, device="cpu"):
+    y = x.detach().to(device).double()
     y = y / (y.square().sum((-2, -1), keepdim=True).sqrt() + eps)
     tall = y.shape[-2] > y.shape[-1]
     if tall:
@@ -29,11 +29,11 @@ def _planes(v, scale):
     return (hi + lo) / scale, hi / scale
 
 
-def modelled(x, wide, steps=5, coefficients=NS, eps=1e-7, sums=None):
+def modelled(x, wide, steps=5, coefficients=NS, eps=1e-7, sums=None, device="cpu"):
     """fp32 accumulation, planes of two fp16 terms (scaled by 2^13, a power of two that keeps every
     value of these tests in range), products of both terms (wide) or of the first (narrow), exact
     diagonals."""
-    y = x.detach().cpu().double()
+    y = x.detach().to(device).double()
     y = (y / (y.square().sum() .sqrt() + eps)).float()
     if y.shape[0] > y.shape[1]:
         y = y.T
