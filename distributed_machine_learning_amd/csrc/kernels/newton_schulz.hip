@@ -163,7 +163,8 @@ __device__ __forceinline__ void ns_load8(const T* p, bool wide, float (&v)[8]) {
 // Partial sums of squares in 64 bits: squares of fp32 values neither overflow nor vanish there.  A
 // wave takes 2048 consecutive elements of a row at a time, and a matrix without gaps between its
 // rows is one long row; 16-byte loads wherever the addresses allow them.  In the update the same
-// pass moves the momentum on.  Memory-bound.
+// pass moves the momentum on.  Memory-bound: 240 MB of a 20 M parameter update in 50 us, 4.8 TB/s (a
+// large copy: 5.2).
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, const T* __restrict__ x, NsUpdate u,
                                                       double* __restrict__ partials) {
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(256) void ns_norm_kernel(NsTable tab, const T* __re
 }
 
 // Y_0 = X / (||X|| + eps) as planes, zeros in the padding.  64 x 64 tiles of the matrix in memory,
-// transposed through LDS where Y is its transpose.
+// transposed through LDS where Y is its transpose.  Memory-bound like the pass before (50 us there).
 template <typename T, bool MUON>
 __global__ __launch_bounds__(256) void ns_load_kernel(NsTable tab, const T* __restrict__ x, NsUpdate u,
                                                       const double* __restrict__ partials, char* ws,
@@ -692,6 +693,11 @@ struct NsSides {
 //     LDS read (per 16 lanes a 4 x 16 block).  32-byte pair p of row k sits at p ^ pair_swizzle(k): the
 //     eight rows that half a wave reads at once meet different banks.
 // The columns' operand is the first of the MFMA, so a lane ends with four consecutive columns of a row.
+//
+// What bounds it: large tiles the matrix units under full load, wide (four of [8192, 2048]: Y Y^T 0.92,
+// B Y 1.0 PFLOP/s; a large library product reaches 1.24), and L2 and LDS traffic, narrow (4096 x 4096:
+// 0.9 PFLOP/s).  64 x 64 tiles read 32 KB of LDS per 16 KB staged, twice the time of their products, but
+// 512 x 512 has only 36 of them for 256 CUs: there latency counts, 11.5 us for 8 steps of PairTile.
 template <typename G, bool WIDE, int PHASE, typename OUT>
 __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void ns_product_kernel(
     NsTable tab, char* ws, float* slab, NsStep s, NsResult res) {
@@ -932,7 +938,7 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
 }
 
 // Adds the parts of split tiles in the order of the summed index and finishes them, a 64 x 64 piece of
-// a tile per block.
+// a tile per block.  Latency of one trip to memory and one back: 6 to 7 us for 36 to 250 tiles.
 template <typename G, int PHASE, typename OUT>
 __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, const float* __restrict__ slab,
                                                       NsStep s, NsResult res) {
