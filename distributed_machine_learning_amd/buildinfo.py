@@ -27,6 +27,10 @@ ARCH = "gfx950:xnack-"
 COMMON_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-fno-gpu-rdc", "-Wall",
                 "-Wno-unused-function", "-D__HIP_PLATFORM_AMD__", "-fno-slp-vectorize"]
 
+# Device code: no packed fp32 VALU instructions at all, also where the compiler forms them from vector
+# code (the host pass does not know the feature and says so).
+DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # Per-file device-code flags.  No -ffast-math anywhere: the kernels call the fast intrinsics
 # they want by name (rsqrtf, __expf) and the reductions rely on a fixed summation order for
 # bit-reproducible training, which reassociation would be free to break.
@@ -38,8 +42,6 @@ FILE_FLAGS = {
     "conv_wgrad.hip": ["-munsafe-fp-atomics"],
     "optim_loss.hip": ["-munsafe-fp-atomics"],
     "conv_f32.hip": ["-munsafe-fp-atomics"],
-    # no packed fp32 VALU instructions at all, also where the compiler forms them from vector code
-    "newton_schulz.hip": ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"],
 }
 
 
@@ -61,7 +63,8 @@ def headers():
 
 
 def flags_for(src: str):
-    return COMMON_FLAGS + FILE_FLAGS.get(os.path.basename(src), [])
+    device = DEVICE_FLAGS if src.endswith(".hip") else []
+    return COMMON_FLAGS + device + FILE_FLAGS.get(os.path.basename(src), [])
 
 
 def digest(paths, extra: str = "") -> str:
@@ -78,4 +81,4 @@ def digest(paths, extra: str = "") -> str:
 
 def tree_hash() -> str:
     """Hash of everything the library is built from: sources, headers, flags."""
-    return digest(sources() + headers(), repr((COMMON_FLAGS, sorted(FILE_FLAGS.items()))))[:32]
+    return digest(sources() + headers(), repr((COMMON_FLAGS, DEVICE_FLAGS, sorted(FILE_FLAGS.items()))))[:32]
