@@ -1097,7 +1097,6 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
 // Latency of barriers and dependent LDS reads bounds it: 64 x 27 takes 21 us, 10 x 512 25, 64 x 448 57
 // (grouped launches: 64 x 520 82), 32 x 1088 51 (32 x 1200 89), 128 x 128 86 (128 x 192 85).
 constexpr int kSoloThreads = 1024, kSoloWaves = kSoloThreads / 64;
-constexpr int kSoloCols = 4096;
 constexpr size_t kSoloLds = 156 * 1024;
 constexpr int kSoloRows = 128;              // largest m
 constexpr int kSoloBatch = 8;               // loads of a thread in flight
@@ -1841,7 +1840,7 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         partials += (long long)p.batch * p.parts;
         if (partials > 0x7fffffffLL) throw std::invalid_argument("newton_schulz: too many matrices");
         sets.back().push_back(p);
-        solo = solo && p.m <= kSoloRows && p.n <= kSoloCols && solo_lds(p.m, p.n) <= kSoloLds;
+        solo = solo && p.m <= kSoloRows && solo_lds(p.m, p.n) <= kSoloLds;
         if (solo) lds = std::max(lds, solo_lds(p.m, p.n));
     }
 

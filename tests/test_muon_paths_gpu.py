@@ -4,7 +4,7 @@ streams on each; matrices whose offsets pass 32 bits."""
 import pytest
 import torch
 
-from support.muon_oracle import exact, gradient, rel, tolerance
+from support.muon_oracle import NS, exact, gradient, rel, tolerance
 from test_muon_gpu import DEV, _muon_oracle, _Net, _wide
 
 pytestmark = pytest.mark.gpu
@@ -34,6 +34,23 @@ def test_sizes(batch, m, n, dtype):
     _close(x, orthogonalize(x))
     x = x.transpose(1, 2).contiguous()
     _close(x, orthogonalize(x))
+
+
+@pytest.mark.parametrize("steps,coefficients", [(1, NS), (2, NS), (3, NS), (4, NS), (6, NS), (8, NS),
+                                                (4, (1.5, -0.5, 0.0)), (5, (1.875, -1.25, 0.375)),
+                                                (3, [(3.0, -3.2, 1.2), (1.875, -1.25, 0.375), (1.5, -0.5, 0.0)])])
+@pytest.mark.parametrize("m,n", [(30, 50), (60, 3000), (200, 6000), (260, 300)])
+def test_steps_and_coefficients(m, n, steps, coefficients):
+    """Steps by themselves and steps that share a product, in runs of every length."""
+    from distributed_machine_learning_amd.optim import orthogonalize
+    x = gradient(m, n, 6).to(DEV)
+    kw = dict(steps=steps, coefficients=coefficients)
+    want = exact(x, device=DEV, **kw)
+    for dtype in KINDS if coefficients is NS else KINDS[:1]:
+        y = orthogonalize(x.to(dtype), **kw)
+        if dtype != torch.float32:
+            want = exact(x.to(dtype), device=DEV, **kw)
+        assert rel(y, want) <= tolerance(x.to(dtype), _wide(dtype, m, n), dtype, device=DEV, **kw)
 
 
 @pytest.mark.parametrize("tall", [False, True])
