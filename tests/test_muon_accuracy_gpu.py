@@ -1,0 +1,38 @@
+"""Newton-Schulz results on inputs whose weak directions drown in the roundings of the strong ones:
+as near to 64 bits as products of fp32 factors, whatever the type."""
+import pytest
+import torch
+
+from support.muon_oracle import exact, rel
+from support.newton_schulz_model import bound, spectra
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+NAMES = sorted(spectra(2, 2))
+# one block per matrix; A A and B Y in one launch; separate launches
+SIZES = [(64, 27), (128, 128), (60, 3000), (128, 1152), (200, 6000), (256, 4096), (512, 4608), (700, 1000)]
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("m,n", SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_default_precision(m, n, dtype, name):
+    from distributed_machine_learning_amd.optim import orthogonalize
+    x = spectra(m, n, 1)[name]
+    x = (x / x.abs().max()).to(dtype).to(DEV)
+    want = exact(x, device=DEV)
+    off, most = rel(orthogonalize(x), want), bound(x, want, dtype, device=DEV)
+    assert off <= most
+
+
+@pytest.mark.parametrize("name", ["low_rank_0.001", "column_1000", "column_100000"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16], ids=["bf16"])
+def test_a_batch_is_as_near_as_its_matrices(dtype, name):
+    from distributed_machine_learning_amd.optim import orthogonalize
+    x = torch.stack([spectra(256, 4096, seed)[name] for seed in range(24)]).to(dtype).to(DEV)
+    y = orthogonalize(x)
+    for i in (0, 11, 23):
+        want = exact(x[i], device=DEV)
+        off, most = rel(y[i], want), bound(x[i], want, dtype, device=DEV)
+        assert off <= most
