@@ -283,8 +283,7 @@ PYBIND11_MODULE(_C, m) {
     py::class_<NewtonSchulzPlan>(m, "NewtonSchulzPlan")
         .def(py::init([](const std::vector<NsTuple>& matrices,
                          const std::vector<std::pair<long long, long long>>& segments,
-                         const std::vector<float>& coefficients, double eps, bool wide_products,
-                         bool fine_result) {
+                         const std::vector<float>& coefficients, double eps, bool wide_products) {
             std::vector<NsShape> shapes;
             for (const NsTuple& t : matrices) {
                 NsShape s;
@@ -294,7 +293,7 @@ PYBIND11_MODULE(_C, m) {
             }
             std::vector<NsSegment> segs;
             for (const auto& g : segments) segs.push_back(NsSegment{g.first, g.second});
-            return new NewtonSchulzPlan(shapes, segs, coefficients, eps, wide_products, fine_result);
+            return new NewtonSchulzPlan(shapes, segs, coefficients, eps, wide_products);
         }))
         .def_property_readonly("workspace_bytes", &NewtonSchulzPlan::workspace_bytes)
         .def("orthogonalize", [](const NewtonSchulzPlan& n, uintptr_t x, uintptr_t out, int type,

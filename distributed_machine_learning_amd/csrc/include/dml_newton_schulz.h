@@ -44,10 +44,9 @@ struct MuonArgs {
 class NewtonSchulzPlan {
   public:
     // `coefficients`: one (a, b, c) per step.  `wide_products`: keep 22 bits of every factor of a
-    // matrix product (two fp16 terms, three products) instead of 11.  `fine_result`: the result
-    // itself is kept in fp32 (an update adds a small multiple of it to the weights).
+    // matrix product (two fp16 terms, three products) instead of 11.
     NewtonSchulzPlan(const std::vector<NsShape>& shapes, const std::vector<NsSegment>& segments,
-                     const std::vector<float>& coefficients, double eps, bool wide_products, bool fine_result);
+                     const std::vector<float>& coefficients, double eps, bool wide_products);
     size_t workspace_bytes() const { return ws_bytes_; }
     // out = NewtonSchulz(x); the workspace (256-byte aligned) holds no state between calls.
     void orthogonalize(const void* x, void* out, NsType type, void* ws, size_t ws_bytes,
@@ -75,7 +74,7 @@ class NewtonSchulzPlan {
     std::vector<NsSegment> segs_;
     std::vector<float> coef_;
     double eps_;
-    bool wide_, squares_wide_ = false, fused_ = false;
+    bool wide_, fused_ = false;
     int x_exp_;                      // Y's planes hold value * 2^exp
     std::vector<std::shared_ptr<Op>> ops_;
     std::shared_ptr<Solo> solo_;

@@ -41,7 +41,7 @@ constexpr int kMaxPartials = 1024;      // blocks (partial sums of squares) per 
 constexpr int kMaxSteps = 64;
 constexpr int kCus = 256;
 
-// Kinds of products: A = Y Y^T; Z = X W of two m x m polynomials in one A; Y <- P Y.
+// Products: A = Y Y^T; P = b A + c A A, its diagonal with the a; Y <- P Y.
 enum NsPhase { GRAM, SQUARE, APPLY };
 
 struct NsProblem {
@@ -69,9 +69,9 @@ static_assert(sizeof(NsTable) <= 3900, "kernel arguments");
 // memory channels (with a power of two they all meet in a few).
 __host__ __device__ inline int ns_pitch(int padded) { return (padded / 64) % 2 ? padded : padded + 64; }
 
-// Workspace of one matrix: Y twice (this product's and the next one's) as [mp, np] planes, the
-// diagonals of the [mp, mp] matrices and their off-diagonal parts as planes.  The hi plane comes first.
-constexpr int kSquares = 5;
+// Workspace of one matrix: Y twice (this step's and the next one's) as [mp, np] planes, the diagonals of
+// A and P and their off-diagonal parts as [mp, mp] planes.  The hi plane comes first.
+enum NsSquare { MAT_A = 0, MAT_P = 1, kSquares = 2 };
 struct NsPlanes {
     uint16_t *y, *squares;
     float* diagonals;
@@ -80,8 +80,8 @@ struct NsPlanes {
     __device__ __forceinline__ uint16_t* square(int i) const { return squares + (size_t)i * 2 * aplane; }
     __device__ __forceinline__ float* diagonal(int i) const { return diagonals + i * mp; }
 };
-inline size_t ns_matrix_bytes(int mp, int np, int squares) {
-    return 8 * (size_t)mp * ns_pitch(np) + 4 * kSquares * (size_t)mp + 4 * squares * (size_t)mp * ns_pitch(mp);
+inline size_t ns_matrix_bytes(int mp, int np) {
+    return 8 * (size_t)mp * ns_pitch(np) + kSquares * (4 * (size_t)mp + 4 * (size_t)mp * ns_pitch(mp));
 }
 __device__ __forceinline__ NsPlanes ns_planes(const NsProblem& q, char* ws, int b, int buffer) {
     NsPlanes r;
@@ -491,9 +491,9 @@ __device__ __forceinline__ NsItem item_of(const NsTable& tab, int block, int blo
 struct NsStep {
     float inv;                  // accumulator -> value
     float sy;                   // Y's planes hold value * sy
-    float ix, iw, sz;           // SQUARE: planes of X, W -> value; value -> planes of Z
-    float k0, k1, k2;           // SQUARE: Z = k0 + k1 X W + k2 W
-    int x, w, z;                // indices of the m x m matrices (GRAM writes z, APPLY multiplies by x)
+    float ia;                   // SQUARE: planes of A -> value
+    float sz;                   // GRAM, SQUARE: value -> planes of A or P
+    float a, b, c;              // SQUARE: P = a + b A + c A A
     int buffer;                 // planes of Y that are read
     int last;                   // APPLY: write the result instead of the next planes
 };
@@ -619,30 +619,25 @@ __device__ __forceinline__ void ns_epilogue(float* E, const float* rows, const f
     } else {
         // Squares of BLOCK above the diagonal are written twice, mirrored the second time; those below
         // it not at all.
-        NsOperand<M, N, THREADS> ox, ow;
-        if constexpr (PHASE == SQUARE) {
-            ow.load(w.square(s.w), w.aplane, w.ald, q.mp, q.mp, i0, j0);
-            ox.load(w.square(s.x), w.aplane, w.ald, q.mp, q.mp, i0, j0);
-        }
+        NsOperand<M, N, THREADS> a;
+        if constexpr (PHASE == SQUARE) a.load(w.square(MAT_A), w.aplane, w.ald, q.mp, q.mp, i0, j0);
         put();
-        uint16_t* dst = w.square(s.z);
-        float* diag = w.diagonal(s.z);
+        constexpr int kTo = PHASE == GRAM ? MAT_A : MAT_P;
+        uint16_t* dst = w.square(kTo);
+        float* diag = w.diagonal(kTo);
 #pragma unroll
         for (int n = 0; n < kTurns; ++n) {
             const int v = threadIdx.x + n * THREADS, r = v / kVec, c = v % kVec * 8, gi = i0 + r, gj = j0 + c;
             if (gi >= q.mp || gj >= q.mp || gj / BLOCK < gi / BLOCK) continue;
-            float z[8], x8[8], w8[8];
-            if (PHASE == SQUARE) {
-                ox.value(n, x8);
-                ow.value(n, w8);
-            }
+            float z[8], a8[8];
+            if (PHASE == SQUARE) a.value(n, a8);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 z[j] = E[r * LD + c + j];
                 if (PHASE == SQUARE) {
-                    const float dx = rows[r], dw = cols[c + j], o = w8[j] * s.iw;
-                    z[j] = gi == gj + j ? s.k1 * (z[j] + dx * dw) + (s.k2 * dw + s.k0)
-                                        : s.k1 * (z[j] + (dx * o + x8[j] * s.ix * dw)) + s.k2 * o;
+                    const float di = rows[r], dj = cols[c + j], o = a8[j] * s.ia;
+                    z[j] = gi == gj + j ? s.c * (z[j] + di * di) + (s.b * di + s.a)
+                                        : s.c * (z[j] + (di + dj) * o) + s.b * o;
                 }
                 if (gi == gj + j) {
                     diag[gi] = z[j];
@@ -672,10 +667,10 @@ __device__ __forceinline__ void ns_epilogue(float* E, const float* rows, const f
 template <int M, int N, int PHASE>
 struct NsSides {
     float row = 0.f, col = 0.f;
-    __device__ __forceinline__ void load(const NsPlanes& w, const NsStep& s, int i0, int j0) {
+    __device__ __forceinline__ void load(const NsPlanes& w, int i0, int j0) {
         const int t = threadIdx.x;
-        if (PHASE != GRAM && t < M && i0 + t < w.mp) row = w.diagonal(s.x)[i0 + t];
-        if (PHASE == SQUARE && t < N && j0 + t < w.mp) col = w.diagonal(s.w)[j0 + t];
+        if (PHASE != GRAM && t < M && i0 + t < w.mp) row = w.diagonal(PHASE == SQUARE ? MAT_A : MAT_P)[i0 + t];
+        if (PHASE == SQUARE && t < N && j0 + t < w.mp) col = w.diagonal(MAT_A)[j0 + t];
     }
     __device__ __forceinline__ void put(float* rows, float* cols) const {
         const int t = threadIdx.x;
@@ -722,13 +717,13 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
     char* ring = smem + group * kRing;
     const int i0 = it.ti * G::kM, j0 = it.tj * G::kN;
     // rows' operand, columns' operand
-    const uint16_t* rp = PHASE == GRAM ? w.y : w.square(s.x);
-    const uint16_t* cp = PHASE == SQUARE ? w.square(s.w) : w.y;
+    const uint16_t* rp = PHASE == GRAM ? w.y : w.square(PHASE == SQUARE ? MAT_A : MAT_P);
+    const uint16_t* cp = PHASE == SQUARE ? w.square(MAT_A) : w.y;
     const size_t rplane = PHASE == GRAM ? w.yplane : w.aplane, cplane = PHASE == SQUARE ? w.aplane : w.yplane;
     const int rld = PHASE == GRAM ? w.yld : w.ald, cld = PHASE == SQUARE ? w.ald : w.yld;
     const int depth = PHASE == GRAM ? q.np : q.mp;
     NsSides<G::kM, G::kN, PHASE> sides;
-    sides.load(w, s, i0, j0);
+    sides.load(w, i0, j0);
 
     int from = 0, to = depth / kStep;
     if (it.split >= 0) {
@@ -958,7 +953,7 @@ __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, con
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, l15 = lane & 15, lq = lane >> 4;
     const NsPlanes w = ns_planes(q, ws, b, s.buffer);
     NsSides<64, 64, PHASE> sides;
-    sides.load(w, s, i0, j0);
+    sides.load(w, i0, j0);
     auto put = [&]() {
         f32x4 sum[4];
 #pragma unroll
@@ -998,7 +993,7 @@ template <bool WIDE, int PHASE>
 __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsTable tab, char* ws, NsStep s) {
     static_assert(PHASE == GRAM || PHASE == SQUARE, "operands along the summed index");
     typedef ShortTile G;
-    constexpr int LD = 36, kPlanes = WIDE ? 2 : 1;
+    constexpr int LD = 36, kPlanes = WIDE ? 2 : 1, kTo = PHASE == GRAM ? MAT_A : MAT_P;
     __shared__ __attribute__((aligned(16))) f32x4 parts[G::kWaves][256];
     __shared__ __attribute__((aligned(16))) float E[32 * LD];
     const NsItem it = item_of<G, PHASE>(tab, blockIdx.x, gridDim.x);
@@ -1006,24 +1001,21 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
     const NsPlanes w = ns_planes(q, ws, it.b, s.buffer);
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63, l15 = lane & 15, lq = lane >> 4;
     const int i0 = it.ti * 32, j0 = it.tj * 32;
-    const uint16_t* rp = PHASE == GRAM ? w.y : w.square(s.x);
-    const uint16_t* cp = PHASE == GRAM ? w.y : w.square(s.w);
+    const uint16_t* x = PHASE == GRAM ? w.y : w.square(MAT_A);
     const size_t plane = PHASE == GRAM ? w.yplane : w.aplane;
     const int ld = PHASE == GRAM ? w.yld : w.ald, depth = PHASE == GRAM ? q.np : q.mp;
 
     // of the first four waves, thread t finishes row fr, columns fc .. fc + 3 (as its accumulators lie)
     const int fr = (t >> 7 & 1) * 16 + l15, fc = (t >> 6 & 1) * 16 + lq * 4;
-    uint2 xh, xl, wh, wl;
-    float dx = 0.f;
-    f32x4 dw;
+    uint2 ah, al;
+    float di = 0.f;
+    f32x4 dj;
     if (PHASE == SQUARE && t < 256) {
         const size_t at = (size_t)(i0 + fr) * ld + j0 + fc;
-        xh = *(const uint2*)(rp + at);
-        xl = *(const uint2*)(rp + plane + at);
-        wh = *(const uint2*)(cp + at);
-        wl = *(const uint2*)(cp + plane + at);
-        dx = w.diagonal(s.x)[i0 + fr];
-        dw = *(const f32x4*)(w.diagonal(s.w) + j0 + fc);
+        ah = *(const uint2*)(x + at);
+        al = *(const uint2*)(x + plane + at);
+        di = w.diagonal(MAT_A)[i0 + fr];
+        dj = *(const f32x4*)(w.diagonal(MAT_A) + j0 + fc);
     }
     f32x4 acc[2][2] = {};
     for (int k = wave * 64; k < depth; k += G::kWaves * 64) {
@@ -1031,30 +1023,30 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int f = 0; f < 2; ++f)
 #pragma unroll
                 for (int l = 0; l < kPlanes; ++l) {
                     const size_t in = (size_t)l * plane + k + h * 32 + lq * 8;
-                    r[h][x][l] = *(const f16x8*)(rp + (size_t)(i0 + x * 16 + l15) * ld + in);
-                    c[h][x][l] = *(const f16x8*)(cp + (size_t)(j0 + x * 16 + l15) * ld + in);
+                    r[h][f][l] = *(const f16x8*)(x + (size_t)(i0 + f * 16 + l15) * ld + in);
+                    c[h][f][l] = *(const f16x8*)(x + (size_t)(j0 + f * 16 + l15) * ld + in);
                 }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int x = 0; x < 2; ++x)
+            for (int f = 0; f < 2; ++f)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
-                    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][0], r[h][x][0], acc[x][y], 0, 0, 0);
+                    acc[f][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][0], r[h][f][0], acc[f][y], 0, 0, 0);
                     if constexpr (WIDE) {
-                        acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][0], r[h][x][1], acc[x][y], 0, 0, 0);
-                        acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][1], r[h][x][0], acc[x][y], 0, 0, 0);
+                        acc[f][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][0], r[h][f][1], acc[f][y], 0, 0, 0);
+                        acc[f][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(c[h][y][1], r[h][f][0], acc[f][y], 0, 0, 0);
                     }
                 }
     }
 #pragma unroll
-    for (int x = 0; x < 2; ++x)
+    for (int f = 0; f < 2; ++f)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) parts[wave][(x * 2 + y) * 64 + lane] = acc[x][y];
+        for (int y = 0; y < 2; ++y) parts[wave][(f * 2 + y) * 64 + lane] = acc[f][y];
     __syncthreads();
     if (t < 256) {
         f32x4 z = parts[0][t];
@@ -1065,13 +1057,12 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (PHASE == SQUARE) {
-                const float o = (f16_value(((const uint16_t*)&wh)[j]) + f16_value(((const uint16_t*)&wl)[j])) * s.iw;
-                const float x = (f16_value(((const uint16_t*)&xh)[j]) + f16_value(((const uint16_t*)&xl)[j])) * s.ix;
-                z[j] = gi == gj + j ? s.k1 * (z[j] + dx * dw[j]) + (s.k2 * dw[j] + s.k0)
-                                    : s.k1 * (z[j] + (dx * o + x * dw[j])) + s.k2 * o;
+                const float o = (f16_value(((const uint16_t*)&ah)[j]) + f16_value(((const uint16_t*)&al)[j])) * s.ia;
+                z[j] = gi == gj + j ? s.c * (z[j] + di * di) + (s.b * di + s.a)
+                                    : s.c * (z[j] + (di + dj[j]) * o) + s.b * o;
             }
             if (gi == gj + j) {
-                w.diagonal(s.z)[gi] = z[j];
+                w.diagonal(kTo)[gi] = z[j];
                 z[j] = 0.f;
             }
         }
@@ -1085,7 +1076,7 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
     uint16_t hi[4], lo[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) split_f16(mirror ? E[(c + j) * LD + r] : E[r * LD + c + j], hi[j], lo[j]);
-    uint16_t* at = w.square(s.z) + (size_t)((mirror ? j0 : i0) + r) * w.ald + (mirror ? i0 : j0) + c;
+    uint16_t* at = w.square(kTo) + (size_t)((mirror ? j0 : i0) + r) * w.ald + (mirror ? i0 : j0) + c;
     *(uint2*)at = *(const uint2*)hi;
     *(uint2*)(at + w.aplane) = *(const uint2*)lo;
 }
@@ -1477,7 +1468,7 @@ __global__ __launch_bounds__(512) void ns_fused_kernel(NsTable tab, char* ws, Ns
 
     // A and a column of Y's tiles to LDS, all loads in flight at once
     constexpr int kA = R * R / 4 / 512, kY = R * 16 / 512;
-    const uint16_t* from = w.square(sq.x);
+    const uint16_t* from = w.square(MAT_A);
     typedef __attribute__((ext_vector_type(4))) unsigned u32x4;
     const int shift = mp == 64 ? 3 : 4;         // 8 or 16 pieces of 16 bytes in a row of A
     u32x4 va[kA], vy[kY];
@@ -1492,7 +1483,7 @@ __global__ __launch_bounds__(512) void ns_fused_kernel(NsTable tab, char* ws, Ns
         const int at = t + n * 512, r = at >> 3, c = (at & 7) * 8, row = r < 2 * mp ? r : 0;
         vy[n] = *(const u32x4*)(w.y + (row >= mp ? w.yplane : 0) + (size_t)(row >= mp ? row - mp : row) * w.yld + j0 + c);
     }
-    const float dt = w.diagonal(sq.x)[t < mp ? t : 0];
+    const float dt = w.diagonal(MAT_A)[t < mp ? t : 0];
 #pragma unroll
     for (int n = 0; n < kA; ++n) {
         const int at = t + n * 512, row = at >> shift, c = (at & ((1 << shift) - 1)) * 8;
@@ -1519,13 +1510,13 @@ __global__ __launch_bounds__(512) void ns_fused_kernel(NsTable tab, char* ws, Ns
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int i = i0 + wr + x * 16 + l15, j = c + lq * 4;
-            const f32x4 o = a.four(i0 + wr + x * 16, c) * sq.iw, dj = *(const f32x4*)(d + j);
+            const f32x4 o = a.four(i0 + wr + x * 16, c) * sq.ia, dj = *(const f32x4*)(d + j);
             const float di = d[i];
             f32x4 z = sum[x].sum() * sq.inv;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                z[r] = i == j + r ? sq.k1 * (z[r] + di * di) + (sq.k2 * di + sq.k0)
-                                  : sq.k1 * (z[r] + (di + dj[r]) * o[r]) + sq.k2 * o[r];
+                z[r] = i == j + r ? sq.c * (z[r] + di * di) + (sq.b * di + sq.a)
+                                  : sq.c * (z[r] + (di + dj[r]) * o[r]) + sq.b * o[r];
                 if (i == j + r) {
                     e[i - i0] = z[r];
                     z[r] = 0.f;
@@ -1758,7 +1749,7 @@ struct NsLaunch {
 }  // namespace
 
 struct NewtonSchulzPlan::Group {
-    NsLaunch norm, load, product[3], wide_square, fused, solo;
+    NsLaunch norm, load, product[3], fused, solo;
     // The workspace of the problem whose partial sums start at `part`, in every table.
     void place(int part, long long ws, long long stride) {
         for (NsTable* t : {&norm.tab, &load.tab, &product[0].tab, &product[1].tab, &product[2].tab,
@@ -1783,7 +1774,7 @@ struct NewtonSchulzPlan::Op {
 NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
                                    const std::vector<NsSegment>& segments,
                                    const std::vector<float>& coefficients, double eps,
-                                   bool wide_products, bool fine_result)
+                                   bool wide_products)
     : segs_(segments), coef_(coefficients), eps_(eps), wide_(wide_products) {
     if (coef_.empty() || coef_.size() % 3 || coef_.size() > 3 * kMaxSteps)
         throw std::invalid_argument("newton_schulz: one (a, b, c) per step, at most 64");
@@ -1803,13 +1794,11 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
 
     // Problems by falling length of their sums: a launch's last blocks are then its cheapest.
     std::vector<NsShape> order = shapes;
-    int smallest = 1 << 30;
     for (const NsShape& s : shapes) {
         if (s.rows <= 0 || s.cols <= 0 || s.batch <= 0 || s.ld < s.cols || s.offset < 0 || s.stride < 0 ||
             s.out_offset < 0)
             throw std::invalid_argument("newton_schulz: bad matrix");
         if (std::max(s.rows, s.cols) > (1 << 24)) throw std::invalid_argument("newton_schulz: dimension over 2^24");
-        smallest = std::min({smallest, s.rows, s.cols});
     }
     std::stable_sort(order.begin(), order.end(), [](const NsShape& x, const NsShape& y) {
         return std::max(x.rows, x.cols) > std::max(y.rows, y.cols);
@@ -1865,102 +1854,47 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         return;
     }
 
-    // Several steps can share one A = Y Y^T and one Y <- P Y: with Q_k = a + b A_k + c A_k^2 the next
-    // step's matrix is A_(k+1) = Q_k A_k Q_k and P the product of the Q_k.  That trades 3 m^2 n
-    // multiplications per step saved for 3 m^3 (symmetric products, always wide), and the rounding of A
-    // grows by a^2 for small singular values with every step that A is carried on: three steps have
-    // 1.4 times the single steps' error at 512 rows, five 70 times (simulated with the planes'
-    // roundings).  Few rows do not average it out: against 64 bits an fp32 result of 32 .. 128 rows is
-    // 1.3 to 6 times as far off as plain fp32 products, one of 192 rows and more 0.9 to 1.15 times.
-    std::vector<int> chains;
-    for (int k = 0; k < steps;) {
-        int n = 1;
-        double growth = 1;
-        while (k + n < steps && n < 3 && !(fine_result && smallest < 192)) {
-            const double a = coef_[3 * (k + n - 1)];
-            growth *= std::max(1.0, a * a);
-            if (growth > 200) break;
-            ++n;
-        }
-        if (n == 3 && steps - k == 4) n = 2;        // 2 + 2 rather than 3 + 1
-        chains.push_back(n);
-        k += n;
-    }
-    double single_us = 0, chain_us = 0, fused_us = 0;
+    double single_us = 0, fused_us = 0;
     bool can_fuse = wide_;
+    size_t slab = 0;
     for (const auto& ps : sets) {
         groups_.push_back(std::make_shared<Group>());
         Group& g = *groups_.back();
         g.norm = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)p.parts; });
         g.load = NsLaunch::simple(ps, [](const NsProblem& p) { return (long long)(p.mp / 64) * (p.np / 64); });
-        for (int phase : {(int)GRAM, (int)SQUARE, (int)APPLY}) g.product[phase] = NsLaunch::product(ps, phase, wide_);
-        g.wide_square = NsLaunch::product(ps, SQUARE, true);
-        const double ends = g.product[GRAM].cost + g.product[APPLY].cost;
-        single_us += steps * (ends + g.product[SQUARE].cost);
-        for (int n : chains) chain_us += ends + (4 * n - 3) * g.wide_square.cost;
+        for (int phase : {(int)GRAM, (int)SQUARE, (int)APPLY}) {
+            g.product[phase] = NsLaunch::product(ps, phase, wide_);
+            slab = std::max(slab, g.product[phase].slab_bytes);
+        }
+        single_us += g.product[SQUARE].cost + g.product[APPLY].cost;
         g.fused = NsLaunch::fused(ps);
         can_fuse = can_fuse && g.fused.blocks;
-        fused_us += steps * (g.product[GRAM].cost + g.fused.cost);
+        fused_us += g.fused.cost;
     }
     fused_ = can_fuse && fused_us < single_us;
-    const bool chained = (int)chains.size() < steps && chain_us < 0.95 * (fused_ ? fused_us : single_us);
-    if (chained) fused_ = false;
-    if (!chained) chains.assign(steps, 1);
-    size_t slab = 0;
-    for (const auto& g : groups_) {
-        if (chained) g->product[SQUARE] = g->wide_square;
-        for (const NsLaunch& l : g->product) slab = std::max(slab, l.slab_bytes);
-    }
-    squares_wide_ = wide_ || chained;
 
-    enum { A = 0, P = 1, P2 = 2, Q = 3, T = 4 };
-    int k = 0, buffer = 0;
-    for (int n : chains) {
-        double amax = sigma[k] * sigma[k], pmax = 1;
-        int ea = scale_exp(std::max(amax, 1e-3)), ep = 0, p = P;
+    // Every step multiplies its own Y.  (Two or three steps could share one A = Y Y^T, carried on as
+    // Q A Q: fewer products where n is several times m, but the rounding of A then grows by a^2 a step
+    // beside a Y that never had it.  With one dominant column that is 2 to 4 times the error of fp32
+    // products for two steps and 10 to 25 times for three; single steps stay at 0.3 to 2.2 times.)
+    for (int k = 0; k < steps; ++k) {
+        const int ea = scale_exp(std::max(sigma[k] * sigma[k], 1e-3)), ep = scale_exp(factor[k]);
         NsStep s{};
         s.sy = std::ldexp(1.f, x_exp_);
-        s.buffer = buffer;
-        auto square = [&](int x, int ex, int w, int ew, int z, int ez, float k0, float k1, float k2) {
-            NsStep t = s;
-            t.inv = std::ldexp(1.f, -ex - ew);
-            t.ix = std::ldexp(1.f, -ex);
-            t.iw = std::ldexp(1.f, -ew);
-            t.sz = std::ldexp(1.f, ez);
-            t.k0 = k0; t.k1 = k1; t.k2 = k2;
-            t.x = x; t.w = w; t.z = z;
-            ops_.push_back(std::make_shared<Op>(Op{SQUARE, t}));
-        };
+        s.buffer = k & 1;
         s.inv = std::ldexp(1.f, -2 * x_exp_);
         s.sz = std::ldexp(1.f, ea);
-        s.z = A;
         ops_.push_back(std::make_shared<Op>(Op{GRAM, s}));
-        for (int i = 0; i < n; ++i, ++k) {
-            const int q = i ? Q : P, eq = scale_exp(factor[k]);
-            square(A, ea, A, ea, q, eq, coef_[3 * k], coef_[3 * k + 2], coef_[3 * k + 1]);
-            if (i + 1 < n) {
-                const int et = scale_exp(std::max(factor[k] * amax, 1e-3));
-                amax = sigma[k + 1] * sigma[k + 1];
-                const int en = scale_exp(std::max(amax, 1e-3));
-                square(q, eq, A, ea, T, et, 0.f, 1.f, 0.f);
-                square(q, eq, T, et, A, en, 0.f, 1.f, 0.f);
-                ea = en;
-            }
-            pmax *= factor[k];
-            if (i) {
-                const int to = p == P ? P2 : P, en = scale_exp(pmax);
-                square(Q, eq, p, ep, to, en, 0.f, 1.f, 0.f);
-                p = to;
-                ep = en;
-            } else {
-                ep = eq;
-            }
-        }
+        s.inv = std::ldexp(1.f, -2 * ea);
+        s.ia = std::ldexp(1.f, -ea);
+        s.sz = std::ldexp(1.f, ep);
+        s.a = coef_[3 * k];
+        s.b = coef_[3 * k + 1];
+        s.c = coef_[3 * k + 2];
+        ops_.push_back(std::make_shared<Op>(Op{SQUARE, s}));
         s.inv = std::ldexp(1.f, -x_exp_ - ep);
-        s.x = p;
-        s.last = k == steps;
+        s.last = k == steps - 1;
         ops_.push_back(std::make_shared<Op>(Op{APPLY, s}));
-        buffer ^= 1;
     }
 
     // workspace: the matrices' planes, the partial sums, the parts of divided tiles
@@ -1968,7 +1902,7 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
     for (size_t i = 0; i < sets.size(); ++i)
         for (size_t j = 0; j < sets[i].size(); ++j) {
             const NsProblem& p = sets[i][j];
-            const size_t each = (ns_matrix_bytes(p.mp, p.np, chained ? kSquares : 2) + 255) & ~(size_t)255;
+            const size_t each = (ns_matrix_bytes(p.mp, p.np) + 255) & ~(size_t)255;
             groups_[i]->place(p.part, (long long)at, (long long)each);
             at += each * p.batch;
         }
@@ -2063,10 +1997,9 @@ void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, cons
                 continue;
             }
             const NsLaunch& l = g->product[op->phase];
-            const bool wide = op->phase == SQUARE ? squares_wide_ : wide_;
             auto go = [&](auto tile) {
                 typedef decltype(tile) G;
-                if (wide) launch_phase<G, true>(l, op->phase, type, ws, slab, op->step, r, stream);
+                if (wide_) launch_phase<G, true>(l, op->phase, type, ws, slab, op->step, r, stream);
                 else launch_phase<G, false>(l, op->phase, type, ws, slab, op->step, r, stream);
             };
             if (l.tile == 0) go(BigTile{});
@@ -2074,7 +2007,7 @@ void NewtonSchulzPlan::chain(char* ws, NsType type, const Prepare& prepare, cons
             else if (l.tile == 2) go(SmallTile{});
             else if (l.tile == 3) go(PairTile{});
             else if (l.tile == 4) launch_apply<HugeTile, false>(l, type, ws, slab, op->step, r, stream);
-            else launch_short(l, op->phase, wide, ws, op->step, stream);
+            else launch_short(l, op->phase, wide_, ws, op->step, stream);
         }
     }
 }

@@ -528,9 +528,9 @@ def _ns_wide(precision: Optional[str]) -> bool:
 
 
 @functools.lru_cache(maxsize=256)
-def _ns_plan(matrices, segments, coefficients, eps, wide, fine):
+def _ns_plan(matrices, segments, coefficients, eps, wide):
     """Plans hold shapes and launch parameters only (no memory), so equal calls share one."""
-    return lib().NewtonSchulzPlan(list(matrices), list(segments), list(coefficients), eps, wide, fine)
+    return lib().NewtonSchulzPlan(list(matrices), list(segments), list(coefficients), eps, wide)
 
 
 def _ns_layout(x: torch.Tensor):
@@ -590,7 +590,7 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     batch, rows, cols, ld, stride, transposed = layout
     out = torch.empty(*x.shape[:-2], rows, cols, dtype=x.dtype, device=x.device)
     plan = _ns_plan(((rows, cols, batch, 0, ld, stride, 0, cols, rows * cols, 0.0),), (), coef,
-                    float(eps), wide, x.dtype == torch.float32)
+                    float(eps), wide)
     with torch.cuda.device(x.device):
         ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=x.device)
         plan.orthogonalize(x.data_ptr(), out.data_ptr(), _NS_TYPES[x.dtype], ws.data_ptr(), ws.numel(),
@@ -620,7 +620,7 @@ class MuonPlan:
         wide = _ns_wide(precision)
         self._plan = lib().NewtonSchulzPlan(
             [(r, c, 1, o, c, 0, 0, 0, 0, f) for o, r, c, f in self.matrices], list(self.segments),
-            list(self.coefficients), self.eps, wide, False)
+            list(self.coefficients), self.eps, wide)
         self.workspace_bytes = int(self._plan.workspace_bytes)
 
 

@@ -1,5 +1,5 @@
 """Newton-Schulz results on inputs whose weak directions drown in the roundings of the strong ones:
-as near to 64 bits as products of fp32 factors, whatever the type."""
+as near to 64 bits as products of fp32 factors, in every type and whatever else is in the batch."""
 import pytest
 import torch
 
@@ -16,7 +16,7 @@ SIZES = [(64, 27), (128, 128), (60, 3000), (128, 1152), (200, 6000), (256, 4096)
 
 @pytest.mark.parametrize("name", NAMES)
 @pytest.mark.parametrize("m,n", SIZES)
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=["fp32", "bf16", "fp16"])
 def test_default_precision(m, n, dtype, name):
     from distributed_machine_learning_amd.optim import orthogonalize
     x = spectra(m, n, 1)[name]
@@ -27,7 +27,7 @@ def test_default_precision(m, n, dtype, name):
 
 
 @pytest.mark.parametrize("name", ["low_rank_0.001", "column_1000", "column_100000"])
-@pytest.mark.parametrize("dtype", [torch.bfloat16], ids=["bf16"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
 def test_a_batch_is_as_near_as_its_matrices(dtype, name):
     from distributed_machine_learning_amd.optim import orthogonalize
     x = torch.stack([spectra(256, 4096, seed)[name] for seed in range(24)]).to(dtype).to(DEV)
@@ -36,3 +36,24 @@ def test_a_batch_is_as_near_as_its_matrices(dtype, name):
         want = exact(x[i], device=DEV)
         off, most = rel(y[i], want), bound(x[i], want, dtype, device=DEV)
         assert off <= most
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_directions_of_an_update(name):
+    """Weights of zero and a step of one: the update is the direction itself, of every matrix of a
+    model of small, long and large ones."""
+    from distributed_machine_learning_amd.ops import native
+    shapes = [(64, 27), (64, 576), (128, 1152), (256, 2304), (512, 4608), (10, 512), (300, 200)]
+    at, matrices = 0, []
+    for m, n in shapes:
+        matrices.append((at, m, n, 1.0))
+        at += -(-m * n // 64) * 64
+    p, g, buf = (torch.zeros(at, device=DEV) for _ in range(3))
+    inputs = [spectra(m, n, 2)[name].to(DEV) for m, n in shapes]
+    for (o, m, n, _), x in zip(matrices, inputs):
+        g[o:o + m * n] = x.flatten()
+    native.muon_step_(native.MuonPlan(matrices, []), p, g, buf, 1.0, 0.0, 0.0)
+    for (o, m, n, _), x in zip(matrices, inputs):
+        want = exact(x, device=DEV)
+        off, most = rel(-p[o:o + m * n].view(m, n), want), bound(x, want, device=DEV)
+        assert off <= most, (m, n)
