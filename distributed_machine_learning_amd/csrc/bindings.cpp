@@ -296,6 +296,13 @@ PYBIND11_MODULE(_C, m) {
             return new NewtonSchulzPlan(shapes, segs, coefficients, eps, wide_products);
         }))
         .def_property_readonly("workspace_bytes", &NewtonSchulzPlan::workspace_bytes)
+        // (kernel, tile, blocks, threads, tiles made whole, tiles joined from parts) each
+        .def_property_readonly("launches", [](const NewtonSchulzPlan& n) {
+            std::vector<std::tuple<std::string, std::string, unsigned, unsigned, unsigned, unsigned>> out;
+            for (const NsLaunchInfo& l : n.launches())
+                out.emplace_back(l.kernel, l.tile, l.blocks, l.threads, l.whole, l.joined);
+            return out;
+        })
         .def("orthogonalize", [](const NewtonSchulzPlan& n, uintptr_t x, uintptr_t out, int type,
                                  uintptr_t ws, size_t ws_bytes, uintptr_t s) {
             if (type < NS_F32 || type > NS_F16) throw std::invalid_argument("newton_schulz: element type");

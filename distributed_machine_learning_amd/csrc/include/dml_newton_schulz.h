@@ -13,6 +13,7 @@
 #include <stdint.h>
 
 #include <memory>
+#include <string>
 #include <vector>
 
 namespace dml {
@@ -41,6 +42,13 @@ struct MuonArgs {
     float grad_scale = 1.f;
 };
 
+// A launch of a plan as it was chosen.
+struct NsLaunchInfo {
+    std::string kernel, tile;
+    unsigned blocks = 0, threads = 0;
+    unsigned whole = 0, joined = 0;      // tiles that one block makes; tiles joined from several blocks' parts
+};
+
 class NewtonSchulzPlan {
   public:
     // `coefficients`: one (a, b, c) per step.  `wide_products`: keep 22 bits of every factor of a
@@ -48,6 +56,8 @@ class NewtonSchulzPlan {
     NewtonSchulzPlan(const std::vector<NsShape>& shapes, const std::vector<NsSegment>& segments,
                      const std::vector<float>& coefficients, double eps, bool wide_products);
     size_t workspace_bytes() const { return ws_bytes_; }
+    // The preparing launches and those of one step, for every set of matrices that shares launches.
+    std::vector<NsLaunchInfo> launches() const;
     // out = NewtonSchulz(x); the workspace (256-byte aligned) holds no state between calls.
     void orthogonalize(const void* x, void* out, NsType type, void* ws, size_t ws_bytes,
                        hipStream_t stream) const;

@@ -17,9 +17,12 @@
 // bits on [512, 4608]: 1e-4 of the result's norm; with the diagonals left in, 3e-3).
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <type_traits>
+#include <utility>
 
 #include "dml_common.h"
 #include "dml_newton_schulz.h"
@@ -447,9 +450,9 @@ struct NsItem {
 // Tiles of the symmetric products: those that touch the upper triangle, column by column.  A column
 // of tiles is kN / kM as wide as it is high, so column j has kN / kM * (j + 1) of them.
 template <typename G>
-__host__ __device__ inline int triangle_tiles(int mp) {
+inline long long triangle_tiles(int mp) {
     constexpr int R = G::kN / G::kM;
-    const int rows = (mp + G::kM - 1) / G::kM, cols = (mp + G::kN - 1) / G::kN;
+    const long long rows = (mp + G::kM - 1) / G::kM, cols = (mp + G::kN - 1) / G::kN;
     return R * cols * (cols - 1) / 2 + rows;
 }
 template <typename G, int PHASE>
@@ -1090,6 +1093,8 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
 constexpr int kSoloThreads = 1024, kSoloWaves = kSoloThreads / 64;
 constexpr size_t kSoloLds = 156 * 1024;
 constexpr int kSoloRows = 128;              // largest m
+constexpr int kSoloMost = 1 << 21;          // blocks of a launch: it has fewer than 2^32 threads
+static_assert((unsigned long long)kSoloMost * kSoloThreads < 1ULL << 32, "threads of a launch");
 constexpr int kSoloBatch = 8;               // loads of a thread in flight
 
 // A matrix in LDS: hi plane, then lo plane.  Addresses are a part that is the same for the wave and one
@@ -1587,8 +1592,11 @@ struct NsLaunch {
     double cost = 0;            // estimate, us
     size_t slab_bytes = 0;
 
+    // A launch has fewer than 2^32 threads, 512 to a block at most (the solo kernel's are counted apart).
+    // No matrices whose workspace a GPU could hold come near it with 64 x 64 tiles.
+    static constexpr long long kMost = (1LL << 23) - 1;
     static int checked(long long blocks) {
-        if (blocks > 0x3fffffffLL) throw std::invalid_argument("newton_schulz: too many blocks");
+        if (blocks > kMost) throw std::invalid_argument("newton_schulz: too many blocks for one launch");
         return (int)blocks;
     }
     template <typename F>
@@ -1630,7 +1638,12 @@ struct NsLaunch {
             return G::kRing ? depth / step : (depth + 511) / 512;
         };
         for (const NsProblem& p : ps) {
-            total += checked(tiles_of<G>(p, phase)) * (long long)p.batch;
+            const long long each = tiles_of<G>(p, phase);
+            if (each > (kMost - total) / p.batch) {     // (too small a tile for matrices of this size)
+                cost = std::numeric_limits<double>::infinity();
+                return l;
+            }
+            total += each * p.batch;
             longest = std::max(longest, steps_of(p));
         }
         // one round of `blocks` with sums of `steps`, `finish`: the share of the tile's own time
@@ -1725,7 +1738,7 @@ struct NsLaunch {
             if (p.mp > kFusedRows) return l;
         double cost;
         l = tiled<SmallTile>(ps, APPLY, true, cost);
-        if (l.join_tiles) return NsLaunch{};
+        if (l.join_tiles || std::isinf(cost)) return NsLaunch{};
         l.cost = kFusedUs * ((l.blocks + kCus - 1) / kCus) + 2.5;
         return l;
     }
@@ -1741,6 +1754,7 @@ struct NsLaunch {
             l[i].tile = i;
             if (cost[i] < cost[best]) best = i;
         }
+        if (std::isinf(cost[best])) throw std::invalid_argument("newton_schulz: too many blocks for one launch");
         l[best].cost = cost[best] + 2.5 + (l[best].join_tiles ? 1.0 : 0.0);
         return l[best];
     }
@@ -1847,7 +1861,25 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
         st.sa = std::ldexp(1.f, scale_exp(amax));
         st.sp = std::ldexp(1.f, scale_exp(*std::max_element(factor.begin(), factor.end())));
         std::copy(coef_.begin(), coef_.end(), st.k);
-        for (const auto& ps : sets) {
+        // a large batch takes several launches
+        std::vector<std::vector<NsProblem>> launches;
+        int blocks = kSoloMost;
+        for (const auto& ps : sets)
+            for (const NsProblem& p : ps)
+                for (int b = 0; b < p.batch;) {
+                    if (blocks == kSoloMost || launches.back().size() == kMaxProblems) {
+                        launches.emplace_back();
+                        blocks = 0;
+                    }
+                    NsProblem part = p;
+                    part.batch = std::min(p.batch - b, kSoloMost - blocks);
+                    part.src += b * p.stride;
+                    part.out += b * p.out_stride;
+                    launches.back().push_back(part);
+                    b += part.batch;
+                    blocks += part.batch;
+                }
+        for (const auto& ps : launches) {
             groups_.push_back(std::make_shared<Group>());
             groups_.back()->solo = NsLaunch::simple(ps, [](const NsProblem&) { return 1LL; });
         }
@@ -1912,6 +1944,28 @@ NewtonSchulzPlan::NewtonSchulzPlan(const std::vector<NsShape>& shapes,
     ws_bytes_ = at + slab;
 }
 
+std::vector<NsLaunchInfo> NewtonSchulzPlan::launches() const {
+    static const struct { const char* name; unsigned threads; } kTiles[6] = {
+        {"128x256", 512}, {"128x128", 256}, {"64x64", 256}, {"64x64 in pairs", 512}, {"256x256", 512}, {"32x32", 512}};
+    std::vector<NsLaunchInfo> out;
+    for (const auto& g : groups_) {
+        if (solo_) {
+            out.push_back({"solo", solo_->rows <= 64 ? "64" : "128", g->solo.blocks, kSoloThreads, 0, 0});
+            continue;
+        }
+        out.push_back({"norm", "", g->norm.blocks, 256, 0, 0});
+        out.push_back({"load", "64x64", g->load.blocks, 256, 0, 0});
+        static const char* const kPhases[3] = {"gram", "square", "apply"};
+        for (int phase = 0; phase < (fused_ ? 1 : 3); ++phase) {
+            const NsLaunch& l = g->product[phase];
+            out.push_back({kPhases[phase], kTiles[l.tile].name, l.blocks, kTiles[l.tile].threads,
+                           (unsigned)l.tab.whole, l.join_tiles});
+        }
+        if (fused_) out.push_back({"square and apply", "64x64", g->fused.blocks, 512, g->fused.blocks, 0});
+    }
+    return out;
+}
+
 void NewtonSchulzPlan::check_workspace(const void* ws, size_t ws_bytes) const {
     if (ws_bytes < ws_bytes_ || ((uintptr_t)ws & 255) || (!ws && ws_bytes_))
         throw std::invalid_argument("newton_schulz: workspace too small or not 256-byte aligned");
@@ -1919,14 +1973,27 @@ void NewtonSchulzPlan::check_workspace(const void* ws, size_t ws_bytes) const {
 
 namespace {
 
+// Launches with the kernel's own parameter types; a launch that is refused raises.
+template <typename... P, typename... A>
+void ns_launch(void (*kernel)(P...), dim3 blocks, unsigned threads, size_t lds, hipStream_t stream, A&&... values) {
+    std::tuple<P...> own(std::forward<A>(values)...);
+    const hipError_t e = std::apply(
+        [&](auto&... v) {
+            void* at[] = {(void*)&v...};
+            return hipLaunchKernel((const void*)kernel, blocks, dim3(threads), at, lds, stream);
+        },
+        own);
+    if (e != hipSuccess) throw std::runtime_error(std::string("newton_schulz: launch: ") + hipGetErrorString(e));
+}
+
 template <typename G, bool WIDE, int PHASE, typename OUT>
 void launch_product(const NsLaunch& l, char* ws, float* slab, const NsStep& s, const NsResult& r,
                     hipStream_t stream) {
-    hipLaunchKernelGGL((ns_product_kernel<G, WIDE, PHASE, OUT>), dim3(l.blocks),
-                       dim3(G::kGroups * G::kWavesM * G::kWavesN * 64), 0, stream, l.tab, ws, slab, s, r);
+    ns_launch(ns_product_kernel<G, WIDE, PHASE, OUT>, l.blocks, G::kGroups * G::kWavesM * G::kWavesN * 64, 0, stream,
+              l.tab, ws, slab, s, r);
     if (l.join_tiles)
-        hipLaunchKernelGGL((ns_join_kernel<G, PHASE, OUT>), dim3(l.join_tiles * (G::kM / 64) * (G::kN / 64)),
-                           dim3(256), 0, stream, l.join, ws, slab, s, r);
+        ns_launch(ns_join_kernel<G, PHASE, OUT>, l.join_tiles * (G::kM / 64) * (G::kN / 64), 256, 0, stream, l.join, ws,
+                  slab, s, r);
 }
 template <typename G, bool WIDE>
 void launch_apply(const NsLaunch& l, NsType type, char* ws, float* slab, const NsStep& s, const NsResult& r,
@@ -1944,15 +2011,13 @@ void launch_phase(const NsLaunch& l, int phase, NsType type, char* ws, float* sl
 }
 void launch_fused(const NsLaunch& l, NsType type, char* ws, const NsStep& square, const NsStep& s, const NsResult& r,
                   hipStream_t stream) {
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(l.blocks), dim3(512), 0, stream, l.tab, ws, square, s, r); };
+    auto go = [&](auto kernel) { ns_launch(kernel, l.blocks, 512, 0, stream, l.tab, ws, square, s, r); };
     if (type == NS_BF16) go(ns_fused_kernel<bf16_t>);
     else if (type == NS_F16) go(ns_fused_kernel<f16_t>);
     else go(ns_fused_kernel<float>);
 }
 void launch_short(const NsLaunch& l, int phase, bool wide, char* ws, const NsStep& s, hipStream_t stream) {
-    auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(l.blocks), dim3(ShortTile::kWaves * 64), 0, stream, l.tab, ws, s);
-    };
+    auto go = [&](auto kernel) { ns_launch(kernel, l.blocks, ShortTile::kWaves * 64, 0, stream, l.tab, ws, s); };
     if (phase == GRAM) go(wide ? ns_short_kernel<true, GRAM> : ns_short_kernel<false, GRAM>);
     else go(wide ? ns_short_kernel<true, SQUARE> : ns_short_kernel<false, SQUARE>);
 }
@@ -1963,12 +2028,11 @@ template <typename T, bool MUON, int ROWS>
 void NewtonSchulzPlan::launch_solo_rows(const Group& g, const void* x, const void* update, const void* result,
                                    hipStream_t stream) const {
     // (more than the default 64 KB of LDS has to be allowed once per device)
-    const void* f = (const void*)ns_solo_kernel<T, MUON, ROWS>;
-    if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kSoloLds) != hipSuccess)
+    const auto kernel = ns_solo_kernel<T, MUON, ROWS>;
+    if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)kSoloLds) != hipSuccess)
         throw std::runtime_error("newton_schulz: hipFuncSetAttribute");
-    hipLaunchKernelGGL((ns_solo_kernel<T, MUON, ROWS>), dim3(g.solo.blocks), dim3(kSoloThreads), solo_->lds, stream,
-                       g.solo.tab, (const T*)x, *(const NsUpdate*)update, eps_, solo_->steps,
-                       *(const NsResult*)result);
+    ns_launch(kernel, g.solo.blocks, kSoloThreads, solo_->lds, stream, g.solo.tab, (const T*)x,
+              *(const NsUpdate*)update, eps_, solo_->steps, *(const NsResult*)result);
 }
 
 template <typename T, bool MUON>
@@ -2020,10 +2084,10 @@ void NewtonSchulzPlan::orthogonalize(const void* x, void* out, NsType type, void
     auto prepare = [&](const Group& g, double* partials, float scale) {
         auto go = [&](auto elem) {
             typedef decltype(elem) T;
-            hipLaunchKernelGGL((ns_norm_kernel<T, false>), dim3(g.norm.blocks), dim3(256), 0, stream,
-                               g.norm.tab, (const T*)x, NsUpdate{}, partials);
-            hipLaunchKernelGGL((ns_load_kernel<T, false>), dim3(g.load.blocks), dim3(256), 0, stream,
-                               g.load.tab, (const T*)x, NsUpdate{}, partials, (char*)ws, eps_, scale);
+            ns_launch(ns_norm_kernel<T, false>, g.norm.blocks, 256, 0, stream, g.norm.tab, (const T*)x, NsUpdate{},
+                      partials);
+            ns_launch(ns_load_kernel<T, false>, g.load.blocks, 256, 0, stream, g.load.tab, (const T*)x, NsUpdate{},
+                      partials, (char*)ws, eps_, scale);
         };
         if (type == NS_BF16) go(bf16_t{});
         else if (type == NS_F16) go(f16_t{});
@@ -2054,16 +2118,16 @@ void NewtonSchulzPlan::muon(float* p, const float* g, float* m, const MuonArgs& 
         }
         const unsigned bx = (unsigned)std::min<long long>((most + 255) / 256, 256);
         if (bx == 0) continue;
-        hipLaunchKernelGGL(ns_segments_kernel, dim3(bx, (unsigned)segs.count), dim3(256), 0, stream, segs,
-                           p, g, m, a.sgd_lr, a.sgd_momentum, a.sgd_weight_decay, a.grad_scale);
+        ns_launch(ns_segments_kernel, dim3(bx, (unsigned)segs.count), 256, 0, stream, segs, p, g, m, a.sgd_lr,
+                  a.sgd_momentum, a.sgd_weight_decay, a.grad_scale);
     }
     if (groups_.empty()) return;
     NsUpdate u{g, m, a.momentum, a.grad_scale, a.nesterov ? 1 : 0};
     auto prepare = [&](const Group& gr, double* partials, float scale) {
-        hipLaunchKernelGGL((ns_norm_kernel<float, true>), dim3(gr.norm.blocks), dim3(256), 0, stream,
-                           gr.norm.tab, (const float*)nullptr, u, partials);
-        hipLaunchKernelGGL((ns_load_kernel<float, true>), dim3(gr.load.blocks), dim3(256), 0, stream,
-                           gr.load.tab, (const float*)nullptr, u, partials, (char*)ws, eps_, scale);
+        ns_launch(ns_norm_kernel<float, true>, gr.norm.blocks, 256, 0, stream, gr.norm.tab, (const float*)nullptr, u,
+                  partials);
+        ns_launch(ns_load_kernel<float, true>, gr.load.blocks, 256, 0, stream, gr.load.tab, (const float*)nullptr, u,
+                  partials, (char*)ws, eps_, scale);
     };
     auto solo = [&](const Group& gr, const NsResult& r) { launch_solo<float, true>(gr, nullptr, &u, &r, stream); };
     chain((char*)ws, NS_F32, prepare, solo, nullptr, p, a.lr, 1.f - a.lr * a.weight_decay, stream);
