@@ -11,10 +11,12 @@ to build it, so a GPU run can never silently use stock torch ops.
 from __future__ import annotations
 
 import functools
+import math
 import os
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from ..config import CIFAR_MEAN, CIFAR_STD
 
@@ -517,7 +519,55 @@ def ns_coefficients(steps: int, coefficients) -> Tuple[float, ...]:
         c = [c] * steps
     if len(c) != steps or any(len(t) != 3 for t in c):
         raise ValueError(f"newton_schulz: coefficients are one (a, b, c) or one for each of the {steps} steps")
-    return tuple(float(v) for t in c for v in t)
+    flat = tuple(float(v) for t in c for v in t)
+    _ns_check_ranges(flat)
+    return flat
+
+
+@functools.lru_cache(maxsize=256)
+def _ns_check_ranges(coefficients: Tuple[float, ...]) -> None:
+    """Singular values start in [0, 1]; values are held in a range that allows for 8 at most, and for
+    1024 of a step's factor ``a + b z + c z^2``.  (The plan makes the same check of its fp32 values.)"""
+    def largest(f, r, squares):
+        """Of |f| over [0, r] at its ends and where its derivative's roots ``squares`` (of x^2) lie in it."""
+        return max(abs(f(x)) for x in [0.0, r] + [math.sqrt(z) for z in squares if 0 < z < r * r])
+
+    values = torch.tensor(coefficients, dtype=torch.float32).tolist()
+    sigma = 1.0
+    for k in range(0, len(values), 3):
+        a, b, c = values[k:k + 3]
+        disc = 9 * b * b - 20 * a * c           # a + 3 b z + 5 c z^2 = 0
+        if c != 0:
+            roots = [(-3 * b + sign * math.sqrt(disc)) / (10 * c) for sign in (-1, 1)] if disc >= 0 else []
+        else:
+            roots = [-a / (3 * b)] if b != 0 else []
+        factor = largest(lambda x: a + x * x * (b + c * x * x), sigma, [-b / (2 * c)] if c != 0 else [])
+        sigma = largest(lambda x: x * (a + x * x * (b + c * x * x)), sigma, roots)
+        if not (sigma <= 8 and factor <= 1024):
+            raise ValueError(f"newton_schulz: step {k // 3} of these coefficients lets singular values grow past 8")
+
+
+def ns_check(x: torch.Tensor, eps: float, precision: Optional[str]) -> None:
+    """What no form of the operator takes, on the CPU or the GPU."""
+    if x.dtype not in _NS_TYPES:
+        raise TypeError(f"newton_schulz: expected fp32, bf16 or fp16, got {x.dtype}")
+    shape = x.shape
+    if len(shape) < 2:
+        raise ValueError(f"newton_schulz: expected [..., m, n], got {tuple(shape)}")
+    ns_check_eps(eps)
+    _ns_wide(precision)
+    m, n = shape[-2:]
+    if m * n and max(m, n) > 1 << 24:
+        raise ValueError(f"newton_schulz: dimension over 2^24 in {tuple(shape)}")
+    if len(shape) > 2 and math.prod(shape[:-2]) >= 1 << 31:
+        raise ValueError(f"newton_schulz: more than 2^31 - 1 matrices in {tuple(shape)}")
+    if forward_ad.unpack_dual(x).tangent is not None:
+        raise ValueError("newton_schulz: has no gradient; x carries a forward-mode tangent")
+
+
+def ns_check_eps(eps: float) -> None:
+    if not (eps >= 0 and math.isfinite(eps)):
+        raise ValueError(f"newton_schulz: eps must be finite and not negative, got {eps}")
 
 
 def _ns_wide(precision: Optional[str]) -> bool:
@@ -562,7 +612,8 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
                   precision: Optional[str] = None) -> torch.Tensor:
     """``Y_0 = x / (||x||_F + eps)``, then ``steps`` times ``Y <- a Y + (b A + c A A) Y`` with
     ``A = Y Y^T`` on the smaller side; ``x`` is ``[..., m, n]`` in fp32, bf16 or fp16 and the
-    result has its shape, type and row / column order.
+    result has its shape, type and row / column order.  Refused are dimensions over 2^24 and
+    coefficients that let singular values, 1 at most at first, grow past 8.
 
     Matrices with contiguous rows or columns and evenly spaced batches are read where they lie,
     any other layout is copied first.  ``precision`` is that of the factors of the products:
@@ -572,10 +623,7 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
     result is off by up to 5e-3 of its norm, a few times the rounding of a bf16 result (1.7e-3)."""
     if not x.is_cuda:
         raise ValueError("newton_schulz: expected a GPU tensor")
-    if x.dtype not in _NS_TYPES:
-        raise TypeError(f"newton_schulz: expected fp32, bf16 or fp16, got {x.dtype}")
-    if x.dim() < 2:
-        raise ValueError(f"newton_schulz: expected [..., m, n], got {tuple(x.shape)}")
+    ns_check(x, eps, precision)
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("newton_schulz: has no gradient; pass x.detach() or call under torch.no_grad()")
     coef = ns_coefficients(steps, coefficients)

@@ -51,12 +51,7 @@ def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=native.NS_COEFFI
     detached from ``x``."""
     if x.is_cuda:
         return native.newton_schulz(x, steps, coefficients, eps, precision)
-    if x.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError(f"orthogonalize: expected fp32, bf16 or fp16, got {x.dtype}")
-    if x.dim() < 2:
-        raise ValueError(f"orthogonalize: expected [..., m, n], got {tuple(x.shape)}")
-    if precision is not None and precision not in native.NS_PRECISIONS:
-        raise ValueError(f"orthogonalize: precision must be one of {native.NS_PRECISIONS}, got {precision!r}")
+    native.ns_check(x, eps, precision)
     return _orthogonalize_cpu(x, native.ns_coefficients(steps, coefficients), float(eps))
 
 
@@ -76,6 +71,7 @@ class Muon:
             else FlatModule(module_or_flat)
         self.lr, self.momentum, self.weight_decay, self.nesterov = lr, momentum, weight_decay, nesterov
         self.sgd_lr, self.sgd_momentum, self.sgd_weight_decay = sgd_lr, sgd_momentum, sgd_weight_decay
+        native.ns_check_eps(eps)
         self.eps, self.precision = float(eps), precision
         self.coefficients = native.ns_coefficients(ns_steps, ns_coefficients)
         self.matrices, self.segments = split_slots(self.flat.slots, sgd_params, adjust_lr_fn)

@@ -26,3 +26,24 @@ def test_a_batch_of_several_launches(order):
     want = exact(x[-1], device=DEV)
     off, most = rel(y[-1], want), bound(x[-1], want, torch.bfloat16, device=DEV)
     assert off <= most
+
+
+def test_refusals_as_on_the_cpu():
+    from torch.autograd import forward_ad
+
+    from distributed_machine_learning_amd.ops import native
+    from distributed_machine_learning_amd.optim import Muon, orthogonalize
+    x = torch.randn(4, 5, device=DEV)
+    for call in (orthogonalize, native.newton_schulz):
+        for kw, what in ((dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(coefficients=(9.0, 0.0, 0.0)), "past 8"),
+                         (dict(precision="bf16"), "precision")):
+            with pytest.raises(ValueError, match=what):
+                call(x, **kw)
+        with forward_ad.dual_level(), pytest.raises(ValueError, match="tangent"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(ValueError, match="2\\^24"):
+            call(x[:1, :1].expand(1, (1 << 24) + 1))
+        with pytest.raises(ValueError, match="matrices"):
+            call(x[:1, :1].expand(1 << 31, 1, 1))
+    with pytest.raises(ValueError, match="eps"):
+        Muon(torch.nn.Linear(4, 5).to(DEV), eps=float("inf"))
