@@ -385,7 +385,7 @@ struct PairTile {       // two groups of 4 waves of 32 x 32, each with half of t
 struct ShortTile {      // 8 waves, each with an eighth of the summed index; a step is 8 x 64 of it
     static constexpr int kM = 32, kN = 32, kWaves = 8, kBlocksPerCu = 2;
     static constexpr bool kRing = false;
-    static constexpr int kGroups = 1, kParts = 1;
+    static constexpr int kGroups = 1;
     static constexpr TileTimes kTimes = {2.0, 0.3, 1.5, {2.5, 3, 0}, {0.5, 0.5, 0}};
 };
 
@@ -1095,7 +1095,6 @@ constexpr size_t kSoloLds = 156 * 1024;
 constexpr int kSoloRows = 128;              // largest m
 constexpr int kSoloMost = 1 << 21;          // blocks of a launch: it has fewer than 2^32 threads
 static_assert((unsigned long long)kSoloMost * kSoloThreads < 1ULL << 32, "threads of a launch");
-constexpr int kSoloBatch = 8;               // loads of a thread in flight
 
 // A matrix in LDS: hi plane, then lo plane.  Addresses are a part that is the same for the wave and one
 // of the lane; `lanes` makes the latter anew, for kept over the steps they crowd out the registers.
