@@ -1,9 +1,13 @@
-"""Newton-Schulz plans without a GPU: the launches that are chosen stay within HIP's limits, and one
-that is refused raises."""
+"""Newton-Schulz plans without a GPU: the launches that are chosen stay within HIP's limits, one
+that is refused raises, and the sizes of the GPU tests take every way through the kernels."""
+import math
+import random
+
 import pytest
 import torch
 
 from distributed_machine_learning_amd.ops import native
+from support.newton_schulz_cases import CASES, chosen
 
 NS = native.ns_coefficients(5, native.NS_COEFFICIENTS)
 
@@ -47,3 +51,27 @@ def test_a_refused_launch_raises(batch, m, n):
     muon = native.MuonPlan([], [(0, 8)])
     with pytest.raises(RuntimeError, match="newton_schulz"):
         muon._plan.muon(*(x.data_ptr() // 16 * 16,) * 3, 0.1, 0.9, 0.0, True, 0.1, 0.9, 0.0, 1.0, 0, 0, 0)
+
+
+@pytest.mark.parametrize("batch,m,n,wide,want", CASES, ids=lambda v: str(v) if not isinstance(v, dict) else "")
+def test_the_way_of_every_case(batch, m, n, wide, want):
+    """What the GPU tests of these sizes run (a changed estimate shows here)."""
+    assert chosen(plan(batch, m, n, wide).launches) == want
+
+
+def test_the_cases_take_every_way():
+    """No plan of 6000 drawn sizes has a launch that no case has."""
+    have = {(kernel, way, wide or kernel == "solo") for _, _, _, wide, want in CASES for kernel, way in want.items()}
+    rng, one = random.Random(5), native.ns_coefficients(1, native.NS_COEFFICIENTS)
+
+    def size(lo, hi):
+        return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+    met = set()
+    for _ in range(6000):
+        m = size(1, 6000)
+        n, batch, wide = size(m, max(m, min(20000, 400_000_000 // m))), size(1, 32) if rng.random() < 0.5 else 1, rng.random() < 0.5
+        if batch * m * n <= 3e7 and batch * m * m <= 3e7:
+            p = native.lib().NewtonSchulzPlan([(m, n, batch, 0, n, m * n, 0, n, m * n, 0.0)], [], list(one), 1e-7, wide)
+            met |= {(kernel, way, wide or kernel == "solo") for kernel, way in chosen(p.launches).items()}
+    assert len(met) > 40 and met <= have, sorted(met - have)
