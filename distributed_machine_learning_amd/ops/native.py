@@ -692,6 +692,8 @@ def muon_step_(plan: MuonPlan, p: torch.Tensor, g: torch.Tensor, m: torch.Tensor
     first, second, third = sorted(t.data_ptr() for t in (p, g, m))
     if p.numel() and min(second - first, third - second) < 4 * p.numel():
         raise ValueError("muon_step_: p, g and m must not overlap")
+    if not plan.elems:
+        return
     if workspace is None:
         workspace = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=p.device)
     else:
