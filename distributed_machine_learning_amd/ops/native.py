@@ -700,6 +700,9 @@ def muon_step_(plan: MuonPlan, p: torch.Tensor, g: torch.Tensor, m: torch.Tensor
         _req(workspace, torch.uint8, "workspace", 1)
         if workspace.numel() < plan.workspace_bytes or workspace.device != p.device:
             raise ValueError(f"muon_step_: workspace of {plan.workspace_bytes} bytes on {p.device} needed")
+        lo, hi = workspace.data_ptr(), workspace.data_ptr() + workspace.numel()
+        if plan.workspace_bytes and any(lo < t.data_ptr() + 4 * t.numel() and t.data_ptr() < hi for t in (p, g, m)):
+            raise ValueError("muon_step_: the workspace must not overlap p, g or m")
     with torch.cuda.device(p.device):
         plan._plan.muon(p.data_ptr(), g.data_ptr(), m.data_ptr(), lr, momentum, weight_decay, nesterov,
                         sgd_lr, sgd_momentum, sgd_weight_decay, grad_scale, workspace.data_ptr(),
