@@ -17,8 +17,8 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
-from ..config import (OPT_MUON, SYNC_ALL_REDUCE, SYNC_DDP, SYNC_GATHER_SCATTER, SYNC_NONE,
-                      TrainConfig)
+from ..config import (OPT_MUON, OPTIMIZERS, SYNC_ALL_REDUCE, SYNC_DDP, SYNC_GATHER_SCATTER,
+                      SYNC_NONE, TrainConfig)
 from ..models.vgg import VGG, VGG_WIDTHS
 from ..ops import native
 from ..optim.muon import split_slots
@@ -43,6 +43,8 @@ class NativeBackend:
         if self.fp32 and cfg.use_graph:
             raise ValueError("--graph replays the bf16 engine's step; the fp32 engine has no "
                              "graph mode")
+        if cfg.optimizer not in OPTIMIZERS:
+            raise ValueError(f"optimizer must be one of {OPTIMIZERS}, got {cfg.optimizer!r}")
         if cfg.optimizer == OPT_MUON and cfg.use_graph:
             raise ValueError("--graph replays the engine's own SGD step; --optimizer muon has no "
                              "graph mode")

@@ -14,8 +14,8 @@ from typing import Dict, Optional, Tuple
 import torch
 import torch.nn.functional as F
 
-from ..config import (OPT_MUON, SYNC_ALL_REDUCE, SYNC_DDP, SYNC_GATHER_SCATTER, SYNC_NONE,
-                      TrainConfig)
+from ..config import (OPT_MUON, OPTIMIZERS, SYNC_ALL_REDUCE, SYNC_DDP, SYNC_GATHER_SCATTER,
+                      SYNC_NONE, TrainConfig)
 from ..models.vgg import VGG
 from ..optim.muon import Muon
 from ..parallel.comm import Communicator
@@ -44,6 +44,8 @@ class TorchBackend:
     loader_layout = "nchw_fp32"
 
     def __init__(self, cfg: TrainConfig, device: torch.device, comm: Optional[Communicator]):
+        if cfg.optimizer not in OPTIMIZERS:
+            raise ValueError(f"optimizer must be one of {OPTIMIZERS}, got {cfg.optimizer!r}")
         self.cfg = cfg
         self.device = device
         self.comm = comm
