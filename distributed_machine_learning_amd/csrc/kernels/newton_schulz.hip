@@ -692,10 +692,12 @@ struct NsSides {
 //     eight rows that half a wave reads at once meet different banks.
 // The columns' operand is the first of the MFMA, so a lane ends with four consecutive columns of a row.
 //
-// What bounds it: large tiles the matrix units under full load, wide (four of [8192, 2048]: Y Y^T 0.92,
-// B Y 1.0 PFLOP/s; a large library product reaches 1.24), and L2 and LDS traffic, narrow (4096 x 4096:
-// 0.9 PFLOP/s).  64 x 64 tiles read 32 KB of LDS per 16 KB staged, twice the time of their products, but
-// 512 x 512 has only 36 of them for 256 CUs: there latency counts, 11.5 us for 8 steps of PairTile.
+// What bounds it: the matrix units with large tiles (wide, eight of [8192, 2048]: Y Y^T 1.02, A A 0.89,
+// B Y 1.08 PFLOP/s, where a large library product reaches 1.24; counters at 4096 x 4096: busy in 62 to 65 %
+// of a CU's cycles, waves waiting in 25 %); narrow, a third of the instructions for the same bytes, B Y of
+// 4096 x 4096 reaches 0.9 PFLOP/s.  With 64 x 64 tiles it is latency: 16 x 512 x 512 keeps the matrix units
+// busy in 19 to 26 % and the LDS in 21 to 27 % of the cycles, and waves wait at barriers and for loads in
+// 35 to 43 %; one 512 x 512 has only 36 tiles for 256 CUs (11.5 us for 8 steps of PairTile).
 template <typename G, bool WIDE, int PHASE, typename OUT>
 __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBlocksPerCu) void ns_product_kernel(
     NsTable tab, char* ws, float* slab, NsStep s, NsResult res) {
@@ -936,7 +938,7 @@ __global__ __launch_bounds__(G::kGroups * G::kWavesM * G::kWavesN * 64, G::kBloc
 }
 
 // Adds the parts of split tiles in the order of the summed index and finishes them, a 64 x 64 piece of
-// a tile per block.  Latency of one trip to memory and one back: 6 to 7 us for 36 to 250 tiles.
+// a tile per block.  Latency of one trip to memory and one back: 6 to 8 us for 36 to 250 tiles of 64 x 64.
 template <typename G, int PHASE, typename OUT>
 __global__ __launch_bounds__(256) void ns_join_kernel(NsTable tab, char* ws, const float* __restrict__ slab,
                                                       NsStep s, NsResult res) {
@@ -1088,8 +1090,10 @@ __global__ __launch_bounds__(ShortTile::kWaves * 64, 4) void ns_short_kernel(NsT
 // Where Y and one m x m matrix fit a CU's LDS, a block runs the whole chain of a matrix by itself:
 // one launch instead of 12 or more, no memory traffic but the matrix itself.  Rows are padded to
 // multiples of 32, pitches by 8 elements so that the 16 rows of a fragment meet different banks.
-// Latency of barriers and dependent LDS reads bounds it: 64 x 27 takes 21 us, 10 x 512 25, 64 x 448 57
-// (grouped launches: 64 x 520 82), 32 x 1088 51 (32 x 1200 89), 128 x 128 86 (128 x 192 85).
+// Latency bounds it: of the 51000 clocks of 64 x 27 waves spend 62 % waiting at barriers and for LDS and
+// memory and 17 % waiting to issue; the matrix units are busy in 2 % and 6 instruction cache lines are
+// missed.  64 x 27 takes 21 us (2.5 a step, 8.8 for launch, norm and planes), 10 x 512 25, 64 x 448 57
+// (grouped launches: 64 x 520 81), 32 x 1056 54 (32 x 1200 89), 128 x 128 86 (128 x 192 85).
 constexpr int kSoloThreads = 1024, kSoloWaves = kSoloThreads / 64;
 constexpr size_t kSoloLds = 156 * 1024;
 constexpr int kSoloRows = 128;              // largest m
@@ -1169,8 +1173,8 @@ struct SoloSteps {
 };
 static_assert(sizeof(NsTable) + sizeof(SoloSteps) <= 4000, "kernel arguments");
 
-// Most of a small matrix's time is instructions that are fetched for the first time, so each piece of code
-// is there once: one loop for both passes over the matrix, one tile of A to a wave where ROWS is 64.
+// One loop for both passes over the matrix, and one tile of A to a wave where ROWS is 64: more copies of
+// the code took the same time.
 template <typename T, bool MUON, int ROWS>
 __global__ __launch_bounds__(kSoloThreads) void ns_solo_kernel(NsTable tab, const T* __restrict__ x, NsUpdate u,
                                                                double eps, SoloSteps st, NsResult res) {
