@@ -1986,7 +1986,9 @@ void ns_launch(void (*kernel)(P...), dim3 blocks, unsigned threads, size_t lds, 
             return hipLaunchKernel((const void*)kernel, blocks, dim3(threads), at, lds, stream);
         },
         own);
-    if (e != hipSuccess) throw std::runtime_error(std::string("newton_schulz: launch: ") + hipGetErrorString(e));
+    if (e == hipSuccess) return;
+    (void)hipGetLastError();        // reported here, not by the next call that looks
+    throw std::runtime_error(std::string("newton_schulz: launch: ") + hipGetErrorString(e));
 }
 
 template <typename G, bool WIDE, int PHASE, typename OUT>

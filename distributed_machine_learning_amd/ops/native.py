@@ -617,8 +617,8 @@ def newton_schulz(x: torch.Tensor, steps: int = 5, coefficients=NS_COEFFICIENTS,
 
     Matrices with contiguous rows or columns and evenly spaced batches are read where they lie,
     any other layout is copied first.  ``precision`` is that of the factors of the products:
-    ``"fp32"`` (the default for every type) keeps 22 bits, ``"fp16"`` 11; sums, Y and the diagonals
-    always keep at least 22.  "fp16" takes a third of the matrix instructions, and loses directions
+    ``"fp32"`` (the default for every type) keeps 22 bits, ``"fp16"`` 11 (22 for matrices that one
+    block takes); sums, Y and the diagonals always keep at least 22.  "fp16" takes a third of the matrix instructions, and loses directions
     that are weaker than about 2^-11 of the strongest: where few directions stand over a low floor its
     result is off by up to 5e-3 of its norm, a few times the rounding of a bf16 result (1.7e-3)."""
     if not x.is_cuda:

@@ -47,8 +47,8 @@ def _orthogonalize_cpu(x: torch.Tensor, coef: Sequence[float], eps: float) -> to
 def orthogonalize(x: torch.Tensor, steps: int = 5, coefficients=native.NS_COEFFICIENTS,
                   eps: float = 1e-7, precision: Optional[str] = None) -> torch.Tensor:
     """Newton-Schulz orthogonalisation of ``[..., m, n]`` matrices (:func:`..ops.native.newton_schulz`
-    has the formula, the layouts and ``precision``).  An update has no gradient: the result is
-    detached from ``x``."""
+    has the formula, the layouts, ``precision`` and what is refused).  An update has no gradient: the
+    result is detached from ``x``, and an ``x`` with a forward-mode tangent is refused."""
     if x.is_cuda:
         return native.newton_schulz(x, steps, coefficients, eps, precision)
     native.ns_check(x, eps, precision)
