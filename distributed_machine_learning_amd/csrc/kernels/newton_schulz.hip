@@ -1580,10 +1580,11 @@ double factor_max(double a, double b, double c, double r) {
     }
     return best;
 }
-// e with v * 2^e in (2^14, 2^15]: half of fp16's range stays free for rounding
+// e with v * 2^e in [2^14, 2^15): half of fp16's range stays free for rounding.  Values under 2^-96
+// are scaled like it (their planes keep fewer bits): 2^e times another scale stays in the range of fp32.
 int scale_exp(double v) {
     int e;
-    std::frexp(v, &e);          // v = f * 2^e, f in [0.5, 1)
+    std::frexp(std::max(v, 0x1p-96), &e);       // v = f * 2^e, f in [0.5, 1)
     return 15 - e;
 }
 

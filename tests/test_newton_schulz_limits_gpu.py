@@ -1,4 +1,6 @@
 """Batches of more matrices than one launch takes."""
+import math
+
 import pytest
 import torch
 
@@ -47,3 +49,22 @@ def test_refusals_as_on_the_cpu():
             call(x[:1, :1].expand(1 << 31, 1, 1))
     with pytest.raises(ValueError, match="eps"):
         Muon(torch.nn.Linear(4, 5).to(DEV), eps=float("inf"))
+
+
+@pytest.mark.parametrize("coefficients", [(0.0, 0.0, 0.0), (1e-38, 0.0, 0.0), (1e-12, 1e-13, 0.0), (-1.0, 0.0, 0.0), (0.0, 0.0, 1e-30)])
+@pytest.mark.parametrize("m,n", [(30, 40), (60, 3000), (200, 300)])
+def test_coefficients_of_almost_nothing(m, n, coefficients):
+    """Factors down to subnormal numbers: no scale of the planes leaves fp32's range (2^141 for 1e-38 did, and 0 times
+    it is no number).  One step, whose first term reaches the result in fp32."""
+    from distributed_machine_learning_amd.optim import orthogonalize
+    x = torch.randn(m, n, generator=torch.Generator().manual_seed(1)).to(DEV)
+    kw = dict(steps=1, coefficients=coefficients)
+    y, want = orthogonalize(x, **kw).double(), exact(x, device=DEV, **kw)
+    # fp32 roundings of normal numbers, half a step of the subnormal ones below 2^-126, and the planes of
+    # P: its factor is bounded by |a| + |b| + |c|, scaled to 2^14 and more, and there the lo plane ends in steps
+    # of 2^-24.  An entry of P is off by half a step, one of P Y by that times the sum over a column of Y,
+    # at most sqrt(m) times the column's norm (an A A of small entries lies that far below the bound of P).
+    scale = 15 - math.frexp(max(sum(map(abs, coefficients)), 2.0 ** -96))[1]
+    planes = 2.0 ** (-25 - scale) * m ** 0.5 * float((x.double() / x.double().norm()).norm(dim=0).max())
+    assert bool(((y - want).abs() <= 2.0 ** -20 * want.abs().max() + 2.0 ** -149 + planes).all())
+    assert bool(torch.isfinite(orthogonalize(x, steps=3, coefficients=coefficients)).all())
